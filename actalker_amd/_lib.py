@@ -201,6 +201,56 @@ class ConvDirectDesc(ctypes.Structure):
     ]
 
 
+class RmsNormDesc(ctypes.Structure):
+    _fields_ = [
+        ("x", c_vp), ("ldx", c_ll),
+        ("res", c_vp), ("ldres", c_ll), ("res_f32", c_int),
+        ("sum", c_vp), ("ldsum", c_ll),
+        ("gamma", c_vp), ("eps", c_float), ("norm", c_int),
+        ("y", c_vp), ("ldy", c_ll), ("eight", c_int),
+        ("scale", c_vp), ("scale_row", c_ll), ("scale_blk", c_ll),
+        ("M", c_int), ("C", c_int),
+    ]
+
+
+class GemmFp8Desc(ctypes.Structure):
+    _fields_ = [
+        ("A", c_vp), ("lda", c_ll), ("ascale", c_vp), ("as_row", c_ll), ("as_blk", c_ll),
+        ("W", c_vp), ("ldw", c_ll), ("wscale", c_vp), ("ws_row", c_ll), ("ws_blk", c_ll),
+        ("bias", c_vp), ("R", c_vp), ("ldr", c_ll),
+        ("C", c_vp), ("ldc", c_ll), ("out_f32", c_int),
+        ("M", c_int), ("N", c_int), ("K", c_int),
+    ]
+
+
+class CausalConvDesc(ctypes.Structure):
+    _fields_ = [
+        ("x", c_vp), ("ldx", c_ll),
+        ("w", c_vp), ("bias", c_vp),
+        ("state", c_vp), ("ld_slot", c_ll),
+        ("starts", c_vp), ("slots", c_vp), ("fresh", c_vp),
+        ("y", c_vp), ("ldy", c_ll),
+        ("T", c_int), ("D", c_int), ("W", c_int), ("nseq", c_int), ("nslots", c_int), ("silu", c_int),
+    ]
+
+
+class SsmScanDesc(ctypes.Structure):
+    _fields_ = [
+        ("u", c_vp), ("ldu", c_ll),
+        ("delta", c_vp), ("ld_delta", c_ll), ("delta_f32", c_int),
+        ("A", c_vp),
+        ("B", c_vp), ("ldb", c_ll), ("C", c_vp), ("ldc", c_ll), ("bc_f32", c_int),
+        ("Dskip", c_vp), ("delta_bias", c_vp),
+        ("z", c_vp), ("ldz", c_ll),
+        ("state", c_vp), ("ld_slot", c_ll),
+        ("starts", c_vp), ("slots", c_vp), ("fresh", c_vp),
+        ("y", c_vp), ("ldy", c_ll),
+        ("T", c_int), ("D", c_int), ("N", c_int), ("G", c_int), ("nseq", c_int), ("nslots", c_int),
+        ("softplus", c_int),
+        ("ws", c_vp), ("ws_bytes", c_ll),
+    ]
+
+
 # Every symbol include/actalker_hip.h declares, with its ctypes signature.
 _P = ctypes.POINTER
 SIGNATURES = {
@@ -226,6 +276,11 @@ SIGNATURES = {
     "acth_selective_scan": ([_P(ScanDesc), c_vp], c_int),
     "acth_selective_scan2": ([_P(ScanDesc), _P(ScanDesc), c_vp], c_int),
     "acth_selective_scan_workspace_size": ([c_int, c_int, c_int, c_int], ctypes.c_size_t),
+    "acth_rmsnorm": ([_P(RmsNormDesc), c_vp], c_int),
+    "acth_gemm_fp8": ([_P(GemmFp8Desc), c_vp], c_int),
+    "acth_causal_conv": ([_P(CausalConvDesc), c_vp], c_int),
+    "acth_ssm_scan": ([_P(SsmScanDesc), c_vp], c_int),
+    "acth_ssm_scan_workspace_size": ([c_int, c_int, c_int, c_int, c_int, c_int], ctypes.c_size_t),
     "acth_conv_direct": ([_P(ConvDirectDesc), c_vp], c_int),
     "acth_softmax_rows": ([c_vp, c_int, c_vp, c_int, c_int, c_int, c_float, c_vp], c_int),
     "acth_timestep_embedding": ([c_vp, c_int, c_int, c_int, c_float, c_float, c_float, c_vp, c_vp], c_int),

@@ -1,0 +1,198 @@
+// Matrix product of e4m3 values with a scale for each block of 128:
+//
+//   C[m][n] = sum_b as[m][b] ws[n / 128][b] sum_{k in block b} A[m][k] W[n][k]  (+ bias[n] + R[m][n])
+//
+// One v_mfma_f32_16x16x128_f8f6f4 covers exactly one block of k, so the scales never enter the matrix unit: each
+// product starts from zero and is added to the fp32 accumulators by one multiply-add a value with the two scales'
+// product. The instruction takes W's rows as its first operand, so a lane's four results are four consecutive columns
+// n of one row m: as[m] is one value a lane, ws one value a tile, and outputs leave as packed rows.
+//
+// Precision. The 8-bit matrix instructions add products in groups of 8 consecutive k and drop what lies below 2^-13 of
+// the group's largest product (toward zero; measured on the card lane by lane, the same for the 32-deep form), which
+// costs up to 7 * 2^-13 of a group's largest product and in practice 2e-6 (signed) to 3e-6 (positive data) of the sum
+// of magnitudes: far below a 16-bit output's half step of 2^-9 or 2^-12. fp32 outputs would show it (1.8e-5 of their
+// norm), so those products go through the 16-bit matrix instructions instead, where e4m3 values are exact and the same
+// sums are off by 1e-9 to 1e-8; that unit runs at half the rate.
+#include "common.h"
+
+namespace {
+
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+
+// 16 x 16 x 128: a lane gives row lane % 16 and 32 bytes of k of each operand; the same bytes are taken from both, so
+// which 32 a lane takes does not matter
+__device__ __forceinline__ f32x4_t mfma8(i32x8_t a, i32x8_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+}
+
+__device__ __forceinline__ i32x8_t frag(const uint8_t* lds, int at0, int at1) {
+  const int4 lo = *reinterpret_cast<const int4*>(lds + at0);
+  const int4 hi = *reinterpret_cast<const int4*>(lds + at1);
+  return (i32x8_t){lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+}
+
+// the 16-bit forms of the 8 bytes at `lds`, exactly
+__device__ __forceinline__ bf16x8_t wide8(const uint8_t* lds) {
+  const int2 v = *reinterpret_cast<const int2*>(lds);
+  bf16x8_t o;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const int x = w ? v.y : v.x;
+#if ACTH_F16
+    const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false);
+    const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true);
+#else
+    const auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false);
+    const auto hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true);
+#endif
+    o[4 * w] = lo[0]; o[4 * w + 1] = lo[1]; o[4 * w + 2] = hi[0]; o[4 * w + 3] = hi[1];
+  }
+  return o;
+}
+
+// bias, residual and store of four consecutive columns [n, n + 4) of row m
+__device__ __forceinline__ void finish4(const ActhGemmFp8Desc& p, int m, int n, f32x4_t v, int vec) {
+  if (m >= p.M) return;
+  if (vec && n + 4 <= p.N) {
+    if (p.bias) {
+      const float4 b = *reinterpret_cast<const float4*>(p.bias + n);
+      v[0] += b.x; v[1] += b.y; v[2] += b.z; v[3] += b.w;
+    }
+    if (p.R) {
+      const uint2 r = *reinterpret_cast<const uint2*>((const bf16_t*)p.R + m * p.ldr + n);
+      v[0] += lo16f(r.x); v[1] += hi16f(r.x); v[2] += lo16f(r.y); v[3] += hi16f(r.y);
+    }
+    if (p.out_f32) *reinterpret_cast<float4*>((float*)p.C + m * p.ldc + n) = make_float4(v[0], v[1], v[2], v[3]);
+    else *reinterpret_cast<uint2*>((bf16_t*)p.C + m * p.ldc + n) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (n + i >= p.N) break;
+    float x = v[i];
+    if (p.bias) x += p.bias[n + i];
+    if (p.R) x += bf2f(((const bf16_t*)p.R)[m * p.ldr + n + i]);
+    if (p.out_f32) ((float*)p.C)[m * p.ldc + n + i] = x;
+    else ((bf16_t*)p.C)[m * p.ldc + n + i] = f2bf(x);
+  }
+}
+
+// 16 bytes from any address: one unaligned load
+__device__ __forceinline__ int4 load16_any(const uint8_t* p) {
+  struct __attribute__((packed, aligned(1))) Any { int v[4]; };
+  const Any a = *reinterpret_cast<const Any*>(p);
+  return make_int4(a.v[0], a.v[1], a.v[2], a.v[3]);
+}
+
+// ---- any sizes, strides and alignment: a 64 x 64 tile, four waves of 32 x 32, one k block at a time through LDS
+template <bool WIDE>
+__global__ __launch_bounds__(256) void gemm_fp8_any_kernel(const ActhGemmFp8Desc p, int vec_out) {
+  constexpr int PITCH = 144;
+  __shared__ __align__(16) uint8_t sa[64 * PITCH], sw[64 * PITCH];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int m0 = blockIdx.x * 64, n0 = blockIdx.y * 64;
+  const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
+  const int r16 = lane & 15, g = lane >> 4;
+  f32x4_t acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[i][j] = (f32x4_t){0, 0, 0, 0};
+
+  const int nkb = (p.K + 127) / 128;
+  for (int kb = 0; kb < nkb; ++kb) {
+    const int k0 = kb * 128;
+    // 64 rows x 8 pieces of 16 bytes for each operand
+    for (int i = tid; i < 512; i += 256) {
+      const int r = i >> 3, c = (i & 7) * 16;
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        const int row = (o ? n0 : m0) + r, rows = o ? p.N : p.M;
+        const uint8_t* src = o ? (const uint8_t*)p.W + row * p.ldw : (const uint8_t*)p.A + row * p.lda;
+        int4 v = make_int4(0, 0, 0, 0);
+        if (row < rows && k0 + c < p.K) {
+          if (k0 + c + 16 <= p.K) {
+            v = load16_any(src + k0 + c);
+          } else {
+            uint32_t b[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (k0 + c + e < p.K) b[e >> 2] |= (uint32_t)src[k0 + c + e] << (8 * (e & 3));
+            v = make_int4((int)b[0], (int)b[1], (int)b[2], (int)b[3]);
+          }
+        }
+        *reinterpret_cast<int4*>((o ? sw : sa) + r * PITCH + c) = v;
+      }
+    }
+    __syncthreads();
+    const float ws = p.wscale[(long long)(n0 >> 7) * p.ws_row + kb * p.ws_blk];
+    float sc[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int ra = m0 + wm + i * 16 + r16;
+      sc[i] = ra < p.M ? p.ascale[(long long)ra * p.as_row + kb * p.as_blk] * ws : 0.0f;
+    }
+    f32x4_t d[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) d[i][j] = (f32x4_t){0, 0, 0, 0};
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        bf16x8_t fa[2], fw[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          fa[i] = wide8(sa + (wm + i * 16 + r16) * PITCH + c * 32 + g * 8);
+          fw[i] = wide8(sw + (wn + i * 16 + r16) * PITCH + c * 32 + g * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) d[i][j] = mfma16x16x32(fw[j], fa[i], d[i][j]);
+      }
+    } else {
+      i32x8_t fa[2], fw[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int ra = (wm + i * 16 + r16) * PITCH, rw = (wn + i * 16 + r16) * PITCH;
+        fa[i] = frag(sa, ra + g * 32, ra + g * 32 + 16);
+        fw[i] = frag(sw, rw + g * 32, rw + g * 32 + 16);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) d[i][j] = mfma8(fw[j], fa[i], d[i][j]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[i][j][e], sc[i], acc[i][j][e]);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) finish4(p, m0 + wm + i * 16 + r16, n0 + wn + j * 16 + g * 4, acc[i][j], vec_out);
+}
+
+bool al(const void* p, long long ld_bytes, int to) { return !p || (((uintptr_t)p | (uintptr_t)ld_bytes) % to) == 0; }
+
+}  // namespace
+
+extern "C" int acth_gemm_fp8(const ActhGemmFp8Desc* d, hipStream_t stream) {
+  if (!d || d->M < 0) return ACTH_EINVAL;
+  if (d->M == 0) return ACTH_OK;
+  if (!d->A || !d->W || !d->C || !d->ascale || !d->wscale || d->N < 1 || d->K < 1) return ACTH_EINVAL;
+  if ((d->M > 1 && (d->lda < d->K || d->ldc < d->N || (d->R && d->ldr < d->N))) || (d->N > 1 && d->ldw < d->K))
+    return ACTH_EINVAL;
+  const int vec_out = al(d->C, d->ldc * (d->out_f32 ? 4 : 2), 16) && al(d->bias, 0, 16) && al(d->R, d->ldr * 2, 8);
+  if (d->N > 65535 * 64) return ACTH_EINVAL;
+  const dim3 grid((unsigned)((d->M + 63) / 64), (unsigned)((d->N + 63) / 64));
+  if (d->out_f32) gemm_fp8_any_kernel<true><<<grid, 256, 0, stream>>>(*d, vec_out);
+  else gemm_fp8_any_kernel<false><<<grid, 256, 0, stream>>>(*d, vec_out);
+  ACTH_CHECK_LAUNCH();
+  return ACTH_OK;
+}

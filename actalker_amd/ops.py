@@ -843,3 +843,374 @@ def softmax_rows(x: torch.Tensor, scale: float, out: Optional[torch.Tensor] = No
     _lib.check(lib.acth_softmax_rows(_p(x), _rows(x, "softmax x"), _p(out), _rows(out, "softmax out"), rows, cols,
                                      float(scale), _stream()), "acth_softmax_rows")
     return out
+
+
+# ------------------------------------------------------------------------------------------
+# The layers of a gated state-space model as they are served: norm, 8-bit products, convolution and scan. Inference
+# only. Every operand lives on one device; the launch goes to that device's current stream.
+FP8 = torch.float8_e4m3fn
+FP8_MAX = 448.0               # the largest e4m3 value
+FP8_BLOCK = 128               # columns (of weights also rows) that share a scale
+FP8_LEAST = 2.0 ** -100       # least block maximum: a block of zeros keeps a scale that can be divided by
+SSM_MAX_STATES = 64
+
+# ACTH_CHECK_ARGS=1: look at device-side sequence offsets and slots on the host (a sync per call)
+_CHECK_ARGS = os.environ.get("ACTH_CHECK_ARGS", "0") == "1"
+
+
+def _served(what: str, *tensors) -> torch.device:
+    """The one device of the operands that are given; refuses CPU tensors, several devices and autograd."""
+    dev = tensors[0].device
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise _lib.ActhError(f"{what}: expected a device tensor, got {t.device}")
+        if t.device != dev:
+            raise _lib.ActhError(f"{what}: operands on {dev} and {t.device}")
+        if grad and t.requires_grad:
+            raise _lib.ActhError(f"{what} has no backward: call it under torch.no_grad() or detach its operands")
+    return dev
+
+
+def _launch_on(dev: torch.device, fn, d, name: str):
+    if dev.index == torch.cuda.current_device():
+        rc = fn(ctypes.byref(d), torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(ctypes.byref(d), torch.cuda.current_stream().cuda_stream)
+    if rc:
+        _lib.check(rc, name)
+
+
+def _mat(t: torch.Tensor, shape, dtype, what: str) -> int:
+    """Checks a (rows, columns) operand with contiguous rows; its row stride."""
+    if t.dtype != dtype:
+        raise _lib.ActhError(f"{what}: expected {dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape) or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise _lib.ActhError(f"{what}: expected a row-major tensor of shape {tuple(shape)}, got {tuple(t.shape)} "
+                             f"strides {t.stride()}")
+    return t.stride(0)
+
+
+def _vec(t: Optional[torch.Tensor], n: int, what: str):
+    """Data pointer of an optional contiguous fp32 vector of n entries."""
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+        raise _lib.ActhError(f"{what}: expected {n} contiguous fp32 entries, got {tuple(t.shape)} {t.dtype}")
+    return t.data_ptr()
+
+
+def _span(t: torch.Tensor):
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _apart(out: torch.Tensor, other: Optional[torch.Tensor], what: str, same_ok: bool = False):
+    """Refuses an output that shares memory with an operand, unless it lies exactly on it (``same_ok``) or the two are
+    different columns of the same rows."""
+    if other is None or not out.numel() or not other.numel():
+        return
+    (a0, a1), (b0, b1) = _span(out), _span(other)
+    if a1 <= b0 or b1 <= a0:
+        return
+    if same_ok and a0 == b0 and out.dtype == other.dtype and out.shape == other.shape and out.stride() == other.stride():
+        return
+    if out.dim() == 2 and other.dim() == 2:
+        pitch = out.stride(0) * out.element_size()
+        wa, wb = out.shape[1] * out.element_size(), other.shape[1] * other.element_size()
+        if pitch == other.stride(0) * other.element_size() and pitch > 0:
+            off = (b0 - a0) % pitch
+            if wa <= off and off + wb <= pitch:
+                return
+    raise _lib.ActhError(f"{what}: the output shares memory with an operand")
+
+
+def _rmsnorm(name, x, gamma, eps, residual, sum_out, out, eight, norm):
+    lib = _lib.load(act_dtype())
+    dev = _served(name, x, gamma, residual, sum_out, out)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise _lib.ActhError(f"{name}: expected x of shape (rows, C), got {tuple(x.shape)}")
+    M, C = x.shape
+    d = _lib.RmsNormDesc()
+    d.x, d.ldx = x.data_ptr(), _mat(x, (M, C), act_dtype(), name + " x")
+    if residual is not None:
+        if residual.dtype not in (torch.float32, act_dtype()):
+            raise _lib.ActhError(f"{name} residual: expected torch.float32 or {act_dtype()}, got {residual.dtype}")
+        d.res, d.ldres = residual.data_ptr(), _mat(residual, (M, C), residual.dtype, name + " residual")
+        d.res_f32 = int(residual.dtype == torch.float32)
+        if sum_out is None:
+            sum_out = torch.empty((M, C), device=dev, dtype=residual.dtype)
+        else:
+            _apart(sum_out, x, name + " sum_out", same_ok=True)
+            _apart(sum_out, residual, name + " sum_out", same_ok=True)
+        d.sum, d.ldsum = sum_out.data_ptr(), _mat(sum_out, (M, C), residual.dtype, name + " sum_out")
+    elif sum_out is not None:
+        raise _lib.ActhError(f"{name}: sum_out without a residual")
+    d.gamma, d.eps, d.norm = _vec(gamma, C, name + " gamma"), float(eps), int(norm)
+    scale = None
+    if eight:
+        # rows start at multiples of 16 bytes and a block's scales lie next to each other, as gemm_fp8 reads them
+        out = torch.empty((M, -(-C // 16) * 16), device=dev, dtype=FP8)[:, :C]
+        kb = -(-C // FP8_BLOCK)
+        scale = torch.empty((kb, M), device=dev, dtype=torch.float32).t()
+        d.y, d.ldy, d.eight = out.data_ptr(), out.stride(0), 1
+        d.scale, d.scale_row, d.scale_blk = scale.data_ptr(), 1, M
+    else:
+        if out is None:
+            out = torch.empty((M, C), device=dev, dtype=act_dtype())
+        else:
+            _apart(out, x, name + " out", same_ok=True)
+            _apart(out, residual, name + " out", same_ok=True)
+            _apart(out, sum_out, name + " out")
+            _apart(out, gamma, name + " out")
+        d.y, d.ldy = out.data_ptr(), _mat(out, (M, C), act_dtype(), name + " out")
+    d.M, d.C = M, C
+    if M:
+        _launch_on(dev, lib.acth_rmsnorm, d, "acth_rmsnorm")
+    res = (out, scale) if eight else (out,)
+    if sum_out is not None:
+        res += (sum_out,)
+    return res if len(res) > 1 else out
+
+
+def rmsnorm(x: torch.Tensor, gamma: Optional[torch.Tensor], eps: float = 1e-5, *,
+            residual: Optional[torch.Tensor] = None, sum_out: Optional[torch.Tensor] = None,
+            out: Optional[torch.Tensor] = None):
+    """Root-mean-square norm of x (rows, C), with the residual's addition: s = x + residual (fp32),
+    y = s / sqrt(mean(s^2) + eps) * gamma. ``gamma`` (C) fp32 or None = 1; ``residual`` fp32 or the activation dtype.
+    Returns y, or (y, s rounded to the residual's dtype) with a residual; ``sum_out`` takes s and may be the residual
+    itself, ``out`` takes y and may be x."""
+    return _rmsnorm("rmsnorm", x, gamma, eps, residual, sum_out, out, False, True)
+
+
+def rmsnorm_fp8(x: torch.Tensor, gamma: Optional[torch.Tensor], eps: float = 1e-5, *,
+                residual: Optional[torch.Tensor] = None, sum_out: Optional[torch.Tensor] = None):
+    """:func:`rmsnorm` with its output in 8 bits: (q, scale), or (q, scale, s) with a residual. q (rows, C) e4m3 and
+    scale (rows, ceil(C / 128)) fp32: y ~ q * scale of its block of 128 columns, scale = max(max|y|, 2^-100) / 448,
+    round to nearest even; a NaN makes its block NaN. Operands of :func:`gemm_fp8`."""
+    return _rmsnorm("rmsnorm_fp8", x, gamma, eps, residual, sum_out, None, True, True)
+
+
+def quant_fp8(x: torch.Tensor):
+    """x (rows, C) in 8 bits with a scale for each row's 128 columns: (q, scale) as :func:`rmsnorm_fp8` gives them,
+    for product operands that no norm makes."""
+    return _rmsnorm("quant_fp8", x, None, 0.0, None, None, None, True, False)
+
+
+def pack_fp8(w: torch.Tensor):
+    """A weight (N, K) for :func:`gemm_fp8`, once at load time: (q e4m3 (N, K), scale fp32 (ceil(N / 128),
+    ceil(K / 128))), a scale for each 128 x 128 block."""
+    w = w.detach().float()
+    if w.dim() != 2 or not w.numel():
+        raise _lib.ActhError(f"pack_fp8: expected a weight of shape (N, K), got {tuple(w.shape)}")
+    N, K = w.shape
+    nb, kb = -(-N // FP8_BLOCK), -(-K // FP8_BLOCK)
+    y = torch.nn.functional.pad(w, (0, kb * FP8_BLOCK - K, 0, nb * FP8_BLOCK - N))
+    y = y.view(nb, FP8_BLOCK, kb, FP8_BLOCK)
+    scale = y.abs().amax(dim=(1, 3)).clamp_min(FP8_LEAST) / FP8_MAX
+    y = (y / scale[:, None, :, None]).clamp(-FP8_MAX, FP8_MAX).view(nb * FP8_BLOCK, kb * FP8_BLOCK)
+    q = torch.zeros((N, -(-K // 16) * 16), device=w.device, dtype=FP8)
+    q[:, :K] = y[:N, :K].to(FP8)
+    return q[:, :K], scale.contiguous()
+
+
+def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
+             bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+             out: Optional[torch.Tensor] = None, out_f32: bool = False) -> torch.Tensor:
+    """out = a . w^T (+ bias + residual) of e4m3 values with a scale for each block of 128: a (M, K) with a_scale
+    (M, ceil(K / 128)) (:func:`rmsnorm_fp8`, :func:`quant_fp8`), w (N, K) with w_scale (ceil(N / 128), ceil(K / 128))
+    (:func:`pack_fp8`), scales fp32 with any strides. fp32 accumulation; ``bias`` (N) fp32, ``residual`` (M, N) in the
+    activation dtype; out in the activation dtype, or fp32 with ``out_f32``. ``out`` may be the residual."""
+    lib = _lib.load(act_dtype())
+    dev = _served("gemm_fp8", a, a_scale, w, w_scale, bias, residual, out)
+    if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1] or w.shape[0] < 1 or w.shape[1] < 1:
+        raise _lib.ActhError(f"gemm_fp8: a {tuple(a.shape)} and w {tuple(w.shape)} do not match")
+    M, K = a.shape
+    N = w.shape[0]
+    kb, nb = -(-K // FP8_BLOCK), -(-N // FP8_BLOCK)
+    d = _lib.GemmFp8Desc()
+    d.A, d.lda = a.data_ptr(), _mat(a, (M, K), FP8, "gemm_fp8 a")
+    d.W, d.ldw = w.data_ptr(), _mat(w, (N, K), FP8, "gemm_fp8 w")
+    for t, shape, what in ((a_scale, (M, kb), "a_scale"), (w_scale, (nb, kb), "w_scale")):
+        if t.dtype != torch.float32 or tuple(t.shape) != shape:
+            raise _lib.ActhError(f"gemm_fp8 {what}: expected fp32 of shape {shape}, got {tuple(t.shape)} {t.dtype}")
+    d.ascale, d.as_row, d.as_blk = a_scale.data_ptr(), a_scale.stride(0), a_scale.stride(1)
+    d.wscale, d.ws_row, d.ws_blk = w_scale.data_ptr(), w_scale.stride(0), w_scale.stride(1)
+    d.bias = _vec(bias, N, "gemm_fp8 bias")
+    if residual is not None:
+        d.R, d.ldr = residual.data_ptr(), _mat(residual, (M, N), act_dtype(), "gemm_fp8 residual")
+    kind = torch.float32 if out_f32 else act_dtype()
+    if out is None:
+        out = torch.empty((M, N), device=dev, dtype=kind)
+    else:
+        for t in (a, a_scale, w, w_scale, bias):
+            _apart(out, t, "gemm_fp8 out")
+        _apart(out, residual, "gemm_fp8 out", same_ok=True)
+    d.C, d.ldc, d.out_f32 = out.data_ptr(), _mat(out, (M, N), kind, "gemm_fp8 out"), int(out_f32)
+    d.M, d.N, d.K = M, N, K
+    if M:
+        _launch_on(dev, lib.acth_gemm_fp8, d, "acth_gemm_fp8")
+    return out
+
+
+def _sequences(name, d, T, nb, starts, slots, fresh, state):
+    """Fills the descriptor's sequence fields (ragged: ``starts``; else nb equal ranges)."""
+    if starts is not None:
+        if starts.dtype != torch.int32 or starts.dim() != 1 or starts.numel() < 2 or not starts.is_contiguous():
+            raise _lib.ActhError(f"{name} starts: expected contiguous int32 row offsets, one more than sequences")
+        d.starts = starts.data_ptr()
+        nb = starts.numel() - 1
+    elif nb < 1 or T % nb:
+        raise _lib.ActhError(f"{name}: {T} rows are not {nb} equal sequences")
+    d.nseq = nb
+    if state is not None:
+        d.nslots = state.shape[0]
+        if slots is None and d.nslots < nb:
+            raise _lib.ActhError(f"{name}: {d.nslots} states for {nb} sequences")
+        if d.nslots < 1:
+            raise _lib.ActhError(f"{name}: the state has no slots")
+    if slots is not None:
+        if state is None:
+            raise _lib.ActhError(f"{name}: slots without a state")
+        if slots.dtype != torch.int32 or tuple(slots.shape) != (nb,) or not slots.is_contiguous():
+            raise _lib.ActhError(f"{name} slots: expected contiguous int32 of {nb} entries")
+        d.slots = slots.data_ptr()
+    if fresh is not None:
+        if fresh.dtype not in (torch.bool, torch.uint8) or tuple(fresh.shape) != (nb,) or not fresh.is_contiguous():
+            raise _lib.ActhError(f"{name} fresh: expected contiguous bool of {nb} entries")
+        d.fresh = fresh.data_ptr()
+    if _CHECK_ARGS:
+        if starts is not None:
+            s = starts.tolist()
+            if s[0] < 0 or s[-1] > T or any(a > b for a, b in zip(s, s[1:])):
+                raise _lib.ActhError(f"{name} starts: offsets must rise from >= 0 to <= {T}")
+        if slots is not None:
+            used = [v for v in slots.tolist() if 0 <= v < d.nslots]
+            if len(set(used)) != len(used):
+                raise _lib.ActhError(f"{name} slots: two sequences share a slot")
+
+
+def causal_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, nb: int = 1,
+                starts: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None,
+                slots: Optional[torch.Tensor] = None, fresh: Optional[torch.Tensor] = None, silu: bool = True,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Short causal convolution of each channel: y[t] = silu(bias + sum_j w[:, j] x[t - W + 1 + j]), W = 2 .. 4 taps.
+    x (T, D) activations, w (D, W) and bias (D) fp32.
+
+    The T rows are ``nb`` equal sequences, or ragged ones: ``starts`` (n + 1) int32 row offsets. ``state``
+    (slots, W - 1, D) holds a sequence's last inputs, oldest first, is read as the rows before the sequence and
+    updated in place; without it sequences start from zeros and nothing is kept. ``slots`` (n) int32: the sequences'
+    places in ``state`` (default 0 .. n - 1; no two alike); a place outside it marks a padding sequence. ``fresh`` (n)
+    bool: start from zeros whatever the state holds. Rows of padding sequences and rows that no sequence holds are left
+    as they were in ``out`` (undefined without one); an empty sequence leaves its state."""
+    name = "causal_conv"
+    lib = _lib.load(act_dtype())
+    dev = _served(name, x, w, bias, state, starts, slots, fresh, out)
+    if x.dim() != 2 or w.dim() != 2 or w.shape[0] != x.shape[1] or x.shape[1] < 1 or not 2 <= w.shape[1] <= 4:
+        raise _lib.ActhError(f"{name}: x {tuple(x.shape)} and w {tuple(w.shape)} (2 to 4 taps)")
+    T, D = x.shape
+    W = w.shape[1]
+    d = _lib.CausalConvDesc()
+    d.x, d.ldx = x.data_ptr(), _mat(x, (T, D), act_dtype(), name + " x")
+    d.w, d.bias = _vec(w, D * W, name + " w"), _vec(bias, D, name + " bias")
+    if state is not None:
+        if state.dtype != act_dtype() or state.dim() != 3 or tuple(state.shape[1:]) != (W - 1, D) or \
+                not state[:1].is_contiguous():
+            raise _lib.ActhError(f"{name} state: expected {act_dtype()} (slots, {W - 1}, {D}), got {tuple(state.shape)} "
+                                 f"{state.dtype} strides {state.stride()}")
+        d.state, d.ld_slot = state.data_ptr(), max(state.stride(0), (W - 1) * D) if state.shape[0] < 2 else state.stride(0)
+        _apart(state, x, name + " state")
+    _sequences(name, d, T, nb, starts, slots, fresh, state)
+    if out is None:
+        out = torch.empty((T, D), device=dev, dtype=act_dtype())
+    else:
+        for t in (x, w, bias, state, starts, slots, fresh):
+            _apart(out, t, name + " out")
+    d.y, d.ldy = out.data_ptr(), _mat(out, (T, D), act_dtype(), name + " out")
+    d.T, d.D, d.W, d.silu = T, D, W, int(silu)
+    if T:
+        _launch_on(dev, lib.acth_causal_conv, d, "acth_causal_conv")
+    return out
+
+
+def causal_conv_step(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, state: torch.Tensor,
+                     slots: Optional[torch.Tensor] = None, fresh: Optional[torch.Tensor] = None, silu: bool = True,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`causal_conv` of one new token of each sequence: x (n, D), row i belongs to sequence i."""
+    return causal_conv(x, w, bias, nb=max(1, x.shape[0]), state=state, slots=slots, fresh=fresh, silu=silu, out=out)
+
+
+def ssm_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
+             D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
+             delta_bias: Optional[torch.Tensor] = None, softplus: bool = True, nb: int = 1,
+             starts: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None,
+             slots: Optional[torch.Tensor] = None, fresh: Optional[torch.Tensor] = None,
+             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Selective scan over kept states: dt = softplus(delta + delta_bias), h = exp(dt A) h + dt u B,
+    y = (sum_n C h + D u) silu(z). u (T, d) activations, delta (T, d) activations or fp32, A (d, N) fp32 with
+    N <= 64, B and C (T, G * N) activations or fp32 (G groups of d / G channels share theirs), D and delta_bias (d)
+    fp32, z (T, d) activations. States and arithmetic in fp32.
+
+    Sequences as in :func:`causal_conv`; ``state`` (slots, d, N) fp32 is where each goes on from, updated in place."""
+    name = "ssm_scan"
+    lib = _lib.load(act_dtype())
+    adt = act_dtype()
+    dev = _served(name, u, delta, A, B, C, D, z, delta_bias, state, starts, slots, fresh, out)
+    if u.dim() != 2 or A.dim() != 2 or B.dim() != 2 or A.shape[0] != u.shape[1] or not 1 <= A.shape[1] <= SSM_MAX_STATES \
+            or u.shape[1] < 1:
+        raise _lib.ActhError(f"{name}: u {tuple(u.shape)}, A {tuple(A.shape)} (1 to {SSM_MAX_STATES} states), "
+                             f"B {tuple(B.shape)}")
+    T, dim = u.shape
+    N = A.shape[1]
+    G = B.shape[1] // N
+    if G < 1 or B.shape[1] % N or dim % G:
+        raise _lib.ActhError(f"{name}: B's {B.shape[1]} columns are not groups of {N} states that divide {dim} channels")
+    if delta.dtype not in (torch.float32, adt) or B.dtype not in (torch.float32, adt):
+        raise _lib.ActhError(f"{name}: delta {delta.dtype} and B {B.dtype} must be torch.float32 or {adt}")
+    d = _lib.SsmScanDesc()
+    d.u, d.ldu = u.data_ptr(), _mat(u, (T, dim), adt, name + " u")
+    d.delta, d.ld_delta = delta.data_ptr(), _mat(delta, (T, dim), delta.dtype, name + " delta")
+    d.delta_f32 = int(delta.dtype == torch.float32)
+    d.A = _vec(A, dim * N, name + " A")
+    d.B, d.ldb = B.data_ptr(), _mat(B, (T, G * N), B.dtype, name + " B")
+    d.C, d.ldc = C.data_ptr(), _mat(C, (T, G * N), B.dtype, name + " C")
+    d.bc_f32 = int(B.dtype == torch.float32)
+    d.Dskip, d.delta_bias = _vec(D, dim, name + " D"), _vec(delta_bias, dim, name + " delta_bias")
+    if z is not None:
+        d.z, d.ldz = z.data_ptr(), _mat(z, (T, dim), adt, name + " z")
+    if state is not None:
+        if state.dtype != torch.float32 or state.dim() != 3 or tuple(state.shape[1:]) != (dim, N) or \
+                not state[:1].is_contiguous():
+            raise _lib.ActhError(f"{name} state: expected fp32 (slots, {dim}, {N}), got {tuple(state.shape)} "
+                                 f"{state.dtype} strides {state.stride()}")
+        d.state, d.ld_slot = state.data_ptr(), max(state.stride(0), dim * N) if state.shape[0] < 2 else state.stride(0)
+    _sequences(name, d, T, nb, starts, slots, fresh, state)
+    if out is None:
+        out = torch.empty((T, dim), device=dev, dtype=adt)
+    else:
+        for t in (u, delta, A, B, C, D, z, delta_bias, state, starts, slots, fresh):
+            _apart(out, t, name + " out")
+    d.y, d.ldy = out.data_ptr(), _mat(out, (T, dim), adt, name + " out")
+    d.T, d.D, d.N, d.G, d.softplus = T, dim, N, G, int(softplus)
+    if T:
+        ws = None
+        need = 0 if starts is None and d.nseq == T else \
+            lib.acth_ssm_scan_workspace_size(T, dim, N, G, d.nseq, int(starts is not None))
+        if need:
+            ws = torch.empty(need // 4, device=dev, dtype=torch.float32)
+            d.ws, d.ws_bytes = ws.data_ptr(), need
+        _launch_on(dev, lib.acth_ssm_scan, d, "acth_ssm_scan")
+        del ws
+    return out
+
+
+def ssm_step(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
+             state: torch.Tensor, D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
+             delta_bias: Optional[torch.Tensor] = None, softplus: bool = True, slots: Optional[torch.Tensor] = None,
+             fresh: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`ssm_scan` of one new token of each sequence: u (n, d), row i belongs to sequence i."""
+    return ssm_scan(u, delta, A, B, C, D=D, z=z, delta_bias=delta_bias, softplus=softplus, nb=max(1, u.shape[0]),
+                    state=state, slots=slots, fresh=fresh, out=out)

@@ -243,6 +243,72 @@ int acth_selective_scan(const ActhScanDesc* d, hipStream_t stream);
 int acth_selective_scan2(const ActhScanDesc* d0, const ActhScanDesc* d1, hipStream_t stream);
 size_t acth_selective_scan_workspace_size(int nb, int G, int D, int nchunks);
 
+/* ---- root-mean-square norm with the residual's addition, 16-bit or 8-bit output (beside acth_layernorm):
+ * s = x + res, sum = s, y = s / sqrt(mean(s^2) + eps) * gamma; with norm = 0, y = s * gamma (quantisation alone).
+ * eight: y holds e4m3 codes, scale[row * scale_row + b * scale_blk] = max(max |y| of columns [128 b, 128 b + 128),
+ * 2^-100) / 448, and a code stands for itself times its block's scale; a NaN in a block makes its scale and codes NaN.
+ * sum may lie exactly on res, y (16-bit) exactly on x. Strides in elements. */
+typedef struct ActhRmsNormDesc {
+  const void* x; long long ldx;
+  const void* res; long long ldres; int res_f32;   /* residual stream, or NULL: fp32 or 16-bit */
+  void* sum; long long ldsum;                      /* updated stream in res's type, or NULL */
+  const float* gamma; float eps; int norm;         /* gamma NULL = 1 */
+  void* y; long long ldy; int eight;
+  float* scale; long long scale_row, scale_blk;
+  int M, C;
+} ActhRmsNormDesc;
+int acth_rmsnorm(const ActhRmsNormDesc* d, hipStream_t stream);
+
+/* ---- matrix product of e4m3 values with a scale for each block of 128 (beside acth_gemm):
+ * C[m][n] = sum_b as[m][b] ws[n / 128][b] sum_{k in block b} A[m][k] W[n][k] (+ bias[n] + R[m][n]), fp32 accumulation.
+ * A (M, K) with a scale per row and 128 columns, W (N, K) with a scale per 128 x 128; K need fill no block.
+ * C in the activation type or fp32. Strides in elements; C and R must not overlap the other operands. */
+typedef struct ActhGemmFp8Desc {
+  const void* A; long long lda; const float* ascale; long long as_row, as_blk;
+  const void* W; long long ldw; const float* wscale; long long ws_row, ws_blk;
+  const float* bias; const void* R; long long ldr;
+  void* C; long long ldc; int out_f32;
+  int M, N, K;
+} ActhGemmFp8Desc;
+int acth_gemm_fp8(const ActhGemmFp8Desc* d, hipStream_t stream);
+
+/* ---- sequences of the two entry points below: nseq ranges of the T token rows. starts (nseq + 1, device, clamped to
+ * [0, T]) or NULL: equal ranges of T / nseq rows. Sequence i keeps its state in slot slots[i] (NULL: i); a slot outside
+ * [0, nslots) marks a padding sequence: its rows are left as they were and it has no state, as are rows that no
+ * sequence holds. A sequence goes on from its slot's state, or from zeros where fresh[i] != 0 (or without a state
+ * tensor), and writes the new state back; an empty one leaves it. Two sequences of a call must not share a slot. */
+
+/* ---- short causal convolution of each channel: y[t] = act(bias + sum_j w[d][j] x[t - W + 1 + j]), W = 2 .. 4; the
+ * state holds a sequence's last W - 1 inputs, oldest first. y must not overlap x. */
+typedef struct ActhCausalConvDesc {
+  const void* x; long long ldx;
+  const float* w; const float* bias;               /* (D, W), (D) or NULL */
+  void* state; long long ld_slot;                  /* (nslots, W - 1, D) 16-bit, or NULL */
+  const int* starts; const int* slots; const unsigned char* fresh;
+  void* y; long long ldy;
+  int T, D, W, nseq, nslots, silu;
+} ActhCausalConvDesc;
+int acth_causal_conv(const ActhCausalConvDesc* d, hipStream_t stream);
+
+/* ---- selective scan over kept states, with gate: dt = softplus(delta + delta_bias) (or delta + delta_bias),
+ * h = exp(dt A) h + dt u B, y = (sum_n C h + Dskip u) silu(z), N <= 64 states, G groups of D / G channels that share
+ * their B and C. fp32 states and arithmetic. y must not overlap u, delta, B, C or z. */
+typedef struct ActhSsmScanDesc {
+  const void* u; long long ldu;
+  const void* delta; long long ld_delta; int delta_f32;
+  const float* A;                                  /* (D, N) */
+  const void* B; long long ldb; const void* C; long long ldc; int bc_f32;   /* rows of G * N */
+  const float* Dskip; const float* delta_bias;     /* (D) or NULL */
+  const void* z; long long ldz;                    /* gate rows, or NULL */
+  float* state; long long ld_slot;                 /* (nslots, D, N), or NULL */
+  const int* starts; const int* slots; const unsigned char* fresh;
+  void* y; long long ldy;
+  int T, D, N, G, nseq, nslots, softplus;
+  float* ws; long long ws_bytes;                   /* acth_ssm_scan_workspace_size bytes, when not 0 */
+} ActhSsmScanDesc;
+int acth_ssm_scan(const ActhSsmScanDesc* d, hipStream_t stream);
+size_t acth_ssm_scan_workspace_size(int T, int D, int N, int G, int nseq, int ragged);
+
 /* ---- direct 3x3 (pad 1, stride 1/2) / temporal (3,1,1) convolution for narrow channel counts
  * (PoseGuider InflatedConv3d, pose_guider.py:17-73; VAE Encoder conv_in / downsamplers, TemporalDecoder
  * conv_in / conv_out / time_conv_out).
