@@ -61,6 +61,13 @@ __device__ __forceinline__ bool seq_kept(const P& p, const Seq& q) {        // d
   return p.state && q.slot >= 0 && !(p.fresh && p.fresh[q.i]);
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
+
+// x / (1 + exp(-x)) with the one-step reciprocal: within 4 roundings of 2^-24, for 16-bit outputs
+__device__ __forceinline__ float silu16(float x) {
+  return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e));
+}
+
 // ------------------------------------------------------------------------------------------------ convolution
 // VEC channels a lane (8: one 16-byte load a row; 1: any width and alignment), a wave 64 x VEC channels of 16 rows. The
 // rows of a tile are loaded before the first is used; the W - 1 rows in front of it are read again (3 of 16, from L2).
@@ -101,7 +108,7 @@ struct ConvLane {
 #pragma unroll
       for (int j = 0; j < W - 1; ++j) a = fmaf(w[j][v], win[j][v], a);
       a = fmaf(w[W - 1][v], x[v], a);
-      y[v] = silu ? silu_f(a) : a;
+      y[v] = silu ? silu16(a) : a;
     }
   }
   static __device__ __forceinline__ void shift(float (*win)[VEC], const float* x) {
@@ -252,26 +259,15 @@ void launch_conv(const ActhCausalConvDesc& d, hipStream_t stream) {
 }
 
 // ------------------------------------------------------------------------------------------------ scan
-constexpr float kLog2e = 1.4426950408889634f;
 
-// softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1], with log1p(e) = 2 atanh(e / (2 + e)) by its series:
-// s = e / (2 + e) <= 1/3, the terms left out add less than s^17 * 2/17 < 1e-9. Relative error a few 2^-24 also where
-// e is small, which log(1 + e) would lose; 16 operations against the 16 x 5 of the states.
+// softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1]. With w = 1 + e rounded and c = e - (w - 1) what the
+// rounding lost, log1p(e) = log(w) + c / w + ..., and c stands for c / w: they differ by at most 2^-25 e, half a step of
+// the result. So small e keep their digits, which log(1 + e) alone would lose, for 7 operations and two of the slow ones.
 __device__ __forceinline__ float softplus16(float x) {
   const float e = __builtin_amdgcn_exp2f(-fabsf(x) * kLog2e);
-  const float d = 2.0f + e;
-  float r = __builtin_amdgcn_rcpf(d);
-  r = fmaf(fmaf(-d, r, 1.0f), r, r);
-  const float s = e * r, q = s * s;
-  float a = fmaf(q, 2.0f / 15.0f, 2.0f / 13.0f);
-  a = fmaf(a, q, 2.0f / 11.0f);
-  a = fmaf(a, q, 2.0f / 9.0f);
-  a = fmaf(a, q, 2.0f / 7.0f);
-  a = fmaf(a, q, 2.0f / 5.0f);
-  a = fmaf(a, q, 2.0f / 3.0f);
-  a = fmaf(a, q, 2.0f);
-  const float v = fmaf(a, s, fmaxf(x, 0.0f));
-  return x != x ? x : v;                             // fmaxf would drop a NaN
+  const float w = 1.0f + e;
+  const float c = e - (w - 1.0f);
+  return fmaxf(x, 0.0f) + fmaf(__builtin_amdgcn_logf(w), 0.69314718055994531f, c);   // NaN passes through e
 }
 
 __device__ __forceinline__ float load_any(const void* p, long long i, int f32) {
@@ -291,19 +287,28 @@ struct Chunks {
   float* s;                                        // (n, D): sums of the time steps
 };
 
-constexpr int TT = 16;                             // rows of a tile in LDS
+constexpr int TT = 8;                             // rows of a tile in LDS
 
 // A wave takes CB channels of a chunk: SPL states a lane, LPC lanes a channel, CPT channels a lane. A tile's time steps
 // (softplus done once, by the staging lane) and inputs dt u sit in LDS as pairs beside the rows of B and C; the output
-// takes the place of the pair that its own lane has just read. One wave a block, so no barrier waits for another wave.
-// Bound: the vector units (per row, channel and state one exponential and four multiply-adds).
-template <int SPL, int LPC, int CPT, bool LOCAL>
-__global__ __launch_bounds__(64) void ssm_scan_kernel(const ActhSsmScanDesc p, const Chunks ck, int vec) {
-  constexpr int CB = 64 / LPC * CPT;
+// takes the place of the pair that its own lane has just read. The next tile's rows are loaded while this one is
+// walked. One wave a block, so no barrier waits for another wave.
+// Channel c of a row lies at place (c % 8)(CB / 8) + c / 8, and rows are CB bytes further apart than they are long:
+// the staging lanes, which hold 8 neighbouring channels each, then write neighbouring places (laid out by channel they
+// met in 4 banks, 16 at a time), and the walking lanes read one place each.
+// Bound: the vector units, a row, channel and state taking one exponential (8 clocks a wave) and four operations (4 each).
+template <int SPL, int LPC, int CPT, bool LOCAL, bool VEC>
+__global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p, const Chunks ck) {
+  constexpr int CL = 64 / LPC;                     // channels a wave holds at once
+  constexpr int CB = CL * CPT;
   constexpr int NS = SPL * LPC;
-  constexpr int E8 = CB * TT / 8 / 64 > 0 ? CB * TT / 8 / 64 : 1;    // 8-channel pieces a lane
-  __shared__ __align__(16) float2 sx[TT][CB];
-  __shared__ __align__(16) float sb[TT][NS], sc[TT][NS];
+  constexpr int C8 = CB / 8;                       // 8-channel pieces a row
+  constexpr int E8 = C8 * TT > 64 ? C8 * TT / 64 : 1;     // pieces a lane
+  constexpr int NB = TT * NS / 64;                 // values of B (and C) a lane
+  constexpr int PITCH = CB + C8;
+  __shared__ __align__(16) float2 sx[TT][PITCH];
+  __shared__ __align__(16) float sb[TT][NS], sc[LOCAL ? 1 : TT][NS];
+  __shared__ __align__(16) float s_bias[CB], s_skip[CB];
   __shared__ int s_ok[TT];
 
   const int lane = threadIdx.x;
@@ -320,16 +325,72 @@ __global__ __launch_bounds__(64) void ssm_scan_kernel(const ActhSsmScanDesc p, c
     if (last.i < 0 || last.i >= p.nseq || last.s >= c1 || last.e <= c1) return;
   }
 
-  const int part = lane % LPC, cl = lane / LPC * CPT;
+  // ---- loads of a tile, held until the tile before it is done. A lane's places move down TT rows a tile. Rows behind
+  // the chunk are not loaded and channels behind the wave's last read that one again: what they leave is never walked
+  // or never stored. States behind the last one keep zeros.
+  uint4 pu[E8], pd[E8][2];
+  uint32_t pb[NB], pc[NB];                         // raw: a conversion here would wait for its load
+  const int dsz = p.delta_f32 ? 4 : 2, bsz = p.bc_f32 ? 4 : 2;
+  const int fr = lane / C8, fd = min(d0 + lane % C8 * 8, d1 - 8);      // (fd: with VEC, d1 - d0 is a multiple of 8)
+  const int gr = lane / NS, gn = lane % NS;
+  const bf16_t* at_u = (const bf16_t*)p.u + (long long)(c0 + fr) * p.ldu + fd;
+  const char* at_d = (const char*)p.delta + ((long long)(c0 + fr) * p.ld_delta + fd) * dsz;
+  const char* at_b = (const char*)p.B + ((long long)(c0 + gr) * p.ldb + g * p.N + gn) * bsz;
+  const char* at_c = (const char*)p.C + ((long long)(c0 + gr) * p.ldc + g * p.N + gn) * bsz;
+#pragma unroll
+  for (int k = 0; k < NB; ++k) pb[k] = pc[k] = 0;
+  auto fetch = [&](int b0) {
+    const int left = c1 - b0;
+    if constexpr (VEC) {
+#pragma unroll
+      for (int k = 0; k < E8; ++k) {
+        const int r = fr + 64 / C8 * k;
+        if (r < TT && r < left) {
+          pu[k] = *reinterpret_cast<const uint4*>(at_u + (long long)(64 / C8 * k) * p.ldu);
+          const uint4* f = reinterpret_cast<const uint4*>(at_d + (long long)(64 / C8 * k) * p.ld_delta * dsz);
+          pd[k][0] = f[0];
+          if (p.delta_f32) pd[k][1] = f[1];
+        }
+      }
+      at_u += (long long)TT * p.ldu;
+      at_d += (long long)TT * p.ld_delta * dsz;
+    }
+    if (gn < p.N) {
+#pragma unroll
+      for (int k = 0; k < NB; ++k)
+        if (gr + 64 / NS * k < left) {
+          const long long ob = (long long)(64 / NS * k) * p.ldb * bsz, oc = (long long)(64 / NS * k) * p.ldc * bsz;
+          if (p.bc_f32) {
+            pb[k] = *reinterpret_cast<const uint32_t*>(at_b + ob);
+            if (!LOCAL) pc[k] = *reinterpret_cast<const uint32_t*>(at_c + oc);
+          } else {
+            pb[k] = *reinterpret_cast<const bf16_t*>(at_b + ob);
+            if (!LOCAL) pc[k] = *reinterpret_cast<const bf16_t*>(at_c + oc);
+          }
+        }
+    }
+    at_b += (long long)TT * p.ldb * bsz;
+    at_c += (long long)TT * p.ldc * bsz;
+  };
+  fetch(c0);
+  for (int c = lane; c < CB; c += 64) {
+    s_bias[c] = p.delta_bias && d0 + c < d1 ? p.delta_bias[d0 + c] : 0.0f;
+    s_skip[c] = p.Dskip && d0 + c < d1 ? p.Dskip[d0 + c] : 0.0f;
+  }
+
+  const int part = lane % LPC;
+  auto place = [&](int j) { return lane / LPC + CL * j; };
+  auto channel = [&](int j) { return d0 + place(j) % C8 * 8 + place(j) / C8; };
   float A[CPT][SPL], h[CPT][SPL], sum[CPT];
 #pragma unroll
   for (int j = 0; j < CPT; ++j) {
     sum[j] = 0.0f;
-    const int d = d0 + cl + j;
+    const int d = channel(j);
 #pragma unroll
     for (int s = 0; s < SPL; ++s) {
       const int n = part * SPL + s;
-      A[j][s] = d < d1 && n < p.N ? p.A[(long long)d * p.N + n] * kLog2e : 0.0f;
+      const float a = p.A[(long long)min(d, d1 - 1) * p.N + min(n, p.N - 1)] * kLog2e;     // loads without branches
+      A[j][s] = n < p.N ? a : 0.0f;
       h[j][s] = 0.0f;
     }
   }
@@ -337,79 +398,89 @@ __global__ __launch_bounds__(64) void ssm_scan_kernel(const ActhSsmScanDesc p, c
 #pragma unroll
     for (int j = 0; j < CPT; ++j)
 #pragma unroll
-      for (int s = 0; s < SPL; ++s) {
-        const int d = d0 + cl + j, n = part * SPL + s;
-        h[j][s] = d < d1 && n < p.N ? from[(long long)d * p.N + n] : 0.0f;
-      }
+      for (int s = 0; s < SPL; ++s) h[j][s] = from[(long long)min(channel(j), d1 - 1) * p.N + min(part * SPL + s, p.N - 1)];
+#pragma unroll
+    for (int j = 0; j < CPT; ++j)
+#pragma unroll
+      for (int s = 0; s < SPL; ++s)
+        if (part * SPL + s >= p.N) h[j][s] = 0.0f;
+  };
+  // every load of a state or of A ends before the walk: left under way, it would make the walk's first use of a state
+  // wait for all loads, the next tile's among them
+  auto pin = [&]() {
+#pragma unroll
+    for (int j = 0; j < CPT; ++j)
+#pragma unroll
+      for (int s = 0; s < SPL; ++s) asm volatile("" : "+v"(h[j][s]), "+v"(A[j][s]));
   };
   auto store_h = [&](float* to) {
 #pragma unroll
     for (int j = 0; j < CPT; ++j)
 #pragma unroll
       for (int s = 0; s < SPL; ++s) {
-        const int d = d0 + cl + j, n = part * SPL + s;
+        const int d = channel(j), n = part * SPL + s;
         if (d < d1 && n < p.N) to[(long long)d * p.N + n] = h[j][s];
       }
   };
   const long long dn = (long long)p.D * p.N;
   if (!LOCAL && q.i >= 0 && q.i < p.nseq && q.s < c0 && q.e > c0) load_h(ck.h + chunk * dn);
+  pin();
 
   int t = c0;
+  __syncthreads();
   for (int b0 = c0; b0 < c1; b0 += TT) {
     const int b1 = min(b0 + TT, c1);
-    // ---- stage the tile
-    float u[E8][8];
+    // ---- the tile into LDS
+    uint4 u[E8], z[E8];
 #pragma unroll
     for (int k = 0; k < E8; ++k) {
-      const int piece = lane + 64 * k;
-      const int r = piece / (CB / 8), c8 = piece % (CB / 8) * 8, d = d0 + c8;
+      const int piece = lane + 64 * k, r = piece / C8, o = piece % C8, d = d0 + o * 8;
+      const long long row = b0 + r;
       const bool in = r < TT && b0 + r < b1;
-      float dl[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { u[k][e] = 0.0f; dl[e] = 0.0f; }
-      if (in && vec && d + 8 <= d1) {
-        const long long row = b0 + r;
-        unpack8(*reinterpret_cast<const uint4*>((const bf16_t*)p.u + row * p.ldu + d), u[k]);
+      float uf[8], dl[8];
+      if constexpr (VEC) {
+        u[k] = pu[k];
         if (p.delta_f32) {
-          const float4* f = reinterpret_cast<const float4*>((const float*)p.delta + row * p.ld_delta + d);
-          const float4 x0 = f[0], x1 = f[1];
-          dl[0] = x0.x; dl[1] = x0.y; dl[2] = x0.z; dl[3] = x0.w; dl[4] = x1.x; dl[5] = x1.y; dl[6] = x1.z; dl[7] = x1.w;
+          dl[0] = __uint_as_float(pd[k][0].x); dl[1] = __uint_as_float(pd[k][0].y);
+          dl[2] = __uint_as_float(pd[k][0].z); dl[3] = __uint_as_float(pd[k][0].w);
+          dl[4] = __uint_as_float(pd[k][1].x); dl[5] = __uint_as_float(pd[k][1].y);
+          dl[6] = __uint_as_float(pd[k][1].z); dl[7] = __uint_as_float(pd[k][1].w);
         } else {
-          unpack8(*reinterpret_cast<const uint4*>((const bf16_t*)p.delta + row * p.ld_delta + d), dl);
+          unpack8(pd[k][0], dl);
         }
-      } else if (in) {
-        const long long row = b0 + r;
+      } else {
+        uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (d + e < d1) {
-            u[k][e] = bf2f(((const bf16_t*)p.u)[row * p.ldu + d + e]);
+        for (int e = 0; e < 8; ++e) {
+          dl[e] = 0.0f;
+          if (in && d + e < d1) {
+            w[e >> 1] |= (uint32_t)((const bf16_t*)p.u)[row * p.ldu + d + e] << (16 * (e & 1));
             dl[e] = load_any(p.delta, row * p.ld_delta + d + e, p.delta_f32);
           }
+        }
+        u[k] = make_uint4(w[0], w[1], w[2], w[3]);
       }
+      unpack8(u[k], uf);
       if (r < TT) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          float x = dl[e];
-          if (p.delta_bias && d + e < d1) x += p.delta_bias[d + e];
+          float x = dl[e] + s_bias[o * 8 + e];
           if (p.softplus) x = softplus16(x);
-          if (!(in && d + e < d1)) x = 0.0f;
-          sx[r][c8 + e] = make_float2(x, x * u[k][e]);
+          sx[r][e * C8 + o] = make_float2(x, x * uf[e]);
         }
       }
+      z[k] = make_uint4(0, 0, 0, 0);
+      if (!LOCAL && p.z && VEC && in && d < d1) z[k] = *reinterpret_cast<const uint4*>((const bf16_t*)p.z + row * p.ldz + d);
     }
-    for (int i = lane; i < TT * NS; i += 64) {
-      const int r = i / NS, n = i % NS;
-      float vb = 0.0f, vc = 0.0f;
-      if (b0 + r < b1 && n < p.N) {
-        const long long row = b0 + r;
-        vb = load_any(p.B, row * p.ldb + g * p.N + n, p.bc_f32);
-        if (!LOCAL) vc = load_any(p.C, row * p.ldc + g * p.N + n, p.bc_f32);
-      }
-      sb[r][n] = vb;
-      if (!LOCAL) sc[r][n] = vc;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const int i = lane + 64 * k;
+      sb[i / NS][i % NS] = p.bc_f32 ? __uint_as_float(pb[k]) : bf2f((bf16_t)pb[k]);
+      if (!LOCAL) sc[i / NS][i % NS] = p.bc_f32 ? __uint_as_float(pc[k]) : bf2f((bf16_t)pc[k]);
     }
     if (!LOCAL && lane < TT) s_ok[lane] = 0;
     __syncthreads();
+    if (b0 + TT < c1) fetch(b0 + TT);
 
     // ---- walk its rows, sequence by sequence
     while (t < b1) {
@@ -426,7 +497,10 @@ __global__ __launch_bounds__(64) void ssm_scan_kernel(const ActhSsmScanDesc p, c
         for (int j = 0; j < CPT; ++j)
 #pragma unroll
           for (int s = 0; s < SPL; ++s) h[j][s] = 0.0f;
-        if (seq_kept(p, q)) load_h(p.state + q.slot * p.ld_slot);
+        if (seq_kept(p, q)) {
+          load_h(p.state + q.slot * p.ld_slot);
+          pin();
+        }
       }
       const int e = min(q.e, b1);
       if (!LOCAL && lane >= t - b0 && lane < e - b0) s_ok[lane] = !p.slots || q.slot >= 0;
@@ -443,22 +517,27 @@ __global__ __launch_bounds__(64) void ssm_scan_kernel(const ActhSsmScanDesc p, c
         }
 #pragma unroll
         for (int j = 0; j < CPT; ++j) {
-          const float2 x = sx[r][cl + j];
+          const float2 x = sx[r][place(j)];
           if (LOCAL) sum[j] += x.x;
+          float y1 = 0.0f;
           y[j] = 0.0f;
 #pragma unroll
           for (int s = 0; s < SPL; ++s) {
             const float a = __builtin_amdgcn_exp2f(x.x * A[j][s]);
             h[j][s] = fmaf(a, h[j][s], x.y * B[s]);
-            if (!LOCAL) y[j] = fmaf(h[j][s], C[s], y[j]);
+            if (!LOCAL) {
+              if (s & 1) y1 = fmaf(h[j][s], C[s], y1);
+              else y[j] = fmaf(h[j][s], C[s], y[j]);
+            }
           }
+          y[j] += y1;
         }
         if (!LOCAL) {
 #pragma unroll
           for (int j = 0; j < CPT; ++j) {
 #pragma unroll
             for (int o = 1; o < LPC; o <<= 1) y[j] += __shfl_xor(y[j], o, 64);
-            if (part == 0) sx[r][cl + j].x = y[j];
+            if (part == 0) sx[r][place(j)].x = y[j];
           }
         }
       }
@@ -477,24 +556,25 @@ __global__ __launch_bounds__(64) void ssm_scan_kernel(const ActhSsmScanDesc p, c
     if (!LOCAL) {
 #pragma unroll
       for (int k = 0; k < E8; ++k) {
-        const int piece = lane + 64 * k;
-        const int r = piece / (CB / 8), c8 = piece % (CB / 8) * 8, d = d0 + c8;
+        const int piece = lane + 64 * k, r = piece / C8, c = piece % C8, d = d0 + c * 8;
         if (r >= TT || !s_ok[r < TT ? r : 0] || d >= d1) continue;
         const long long row = b0 + r;
-        const bool full = vec && d + 8 <= d1;
-        float y[8], z[8];
-        if (p.z && full) unpack8(*reinterpret_cast<const uint4*>((const bf16_t*)p.z + row * p.ldz + d), z);
+        float y[8], uf[8], zf[8];
+        unpack8(u[k], uf);
+        unpack8(z[k], zf);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          y[e] = 0.0f;
-          if (d + e < d1) {
-            y[e] = sx[r][c8 + e].x;
-            if (p.Dskip) y[e] = fmaf(p.Dskip[d + e], u[k][e], y[e]);
-            if (p.z) y[e] *= silu_f(full ? z[e] : bf2f(((const bf16_t*)p.z)[row * p.ldz + d + e]));
-          }
+          y[e] = sx[r][e * C8 + c].x;
+          if (p.Dskip) y[e] = fmaf(s_skip[c * 8 + e], uf[e], y[e]);
+          if (p.z && VEC) y[e] *= silu16(zf[e]);
+        }
+        if (p.z && !VEC) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (d + e < d1) y[e] *= silu16(bf2f(((const bf16_t*)p.z)[row * p.ldz + d + e]));
         }
         bf16_t* o = (bf16_t*)p.y + row * p.ldy + d;
-        if (full) {
+        if constexpr (VEC) {
           *reinterpret_cast<uint4*>(o) = pack8(y);
         } else {
 #pragma unroll
@@ -510,7 +590,7 @@ __global__ __launch_bounds__(64) void ssm_scan_kernel(const ActhSsmScanDesc p, c
     if (part == 0) {
 #pragma unroll
       for (int j = 0; j < CPT; ++j)
-        if (d0 + cl + j < d1) ck.s[(long long)chunk * p.D + d0 + cl + j] = sum[j];
+        if (channel(j) < d1) ck.s[(long long)chunk * p.D + channel(j)] = sum[j];
     }
   }
 }
@@ -534,18 +614,22 @@ __global__ __launch_bounds__(256) void ssm_carry_kernel(const ActhSsmScanDesc p,
     }
     __syncthreads();
     const int n = min(256, ck.n - 1 - b);
-#pragma unroll 8
-    for (int k = 0; k < n; ++k) {
-      const int kind = s_kind[k];
-      const long long at = (long long)(b + k);
-      if (kind) {
-        const float e = ck.h[at * dn + ii], s = ck.s[at * p.D + d];
-        const float keep = kind == 2 ? __builtin_amdgcn_exp2f(A * s) * h : 0.0f;
-        if (i < dn) ck.h[at * dn + ii] = h;
-        h = keep + e;
-      } else {
-        if (i < dn) ck.h[at * dn + ii] = h;
-        h = 0.0f;
+    // loads of 8 chunks at a time, whatever their kind, so that they are all under way together
+    for (int k = 0; k < n; k += 8) {
+      float e[8], s[8];
+#pragma unroll
+      for (int v = 0; v < 8; ++v) {
+        const long long at = b + min(k + v, n - 1);
+        e[v] = ck.h[at * dn + ii];
+        s[v] = ck.s[at * p.D + d];
+      }
+#pragma unroll
+      for (int v = 0; v < 8; ++v) {
+        if (k + v >= n) break;
+        const int kind = s_kind[k + v];
+        if (i < dn) ck.h[(b + k + v) * dn + ii] = h;
+        const float keep = kind == 2 ? __builtin_amdgcn_exp2f(A * s[v]) * h : 0.0f;
+        h = kind ? keep + e[v] : 0.0f;
       }
     }
   }
@@ -557,8 +641,12 @@ __global__ __launch_bounds__(256) void ssm_keep_kernel(const ActhSsmScanDesc p, 
   const int c = blockIdx.y, c0 = c * ck.len, c1 = min(c0 + ck.len, p.T);
   const Seq q = seq_find(p, c0);
   if (q.i < 0 || q.i >= p.nseq || q.s >= c0 || q.e <= c0 || q.e > c1 || q.slot < 0) return;
-  const long long dn = (long long)p.D * p.N, i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i < dn) p.state[q.slot * p.ld_slot + i] = ck.h[c * dn + i];
+  const long long dn = (long long)p.D * p.N;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const long long i = ((long long)blockIdx.x * 16 + k) * 256 + threadIdx.x;
+    if (i < dn) p.state[q.slot * p.ld_slot + i] = ck.h[c * dn + i];
+  }
 }
 
 // One row a sequence: a lane holds VN states of one channel (VN = 4: a 16-byte load), LPC lanes a channel, and takes
@@ -612,7 +700,7 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(const ActhSsmScanDesc p, 
     }
     if (in && part == 0) {
       y = fmaf(skip, u, y);
-      if (p.z) y *= silu_f(bf2f(((const bf16_t*)p.z)[row * p.ldz + dd]));
+      if (p.z) y *= silu16(bf2f(((const bf16_t*)p.z)[row * p.ldz + dd]));
       ((bf16_t*)p.y)[row * p.ldy + dd] = f2bf(y);
     }
   }
@@ -638,10 +726,10 @@ Chunks plan(int T, int D, int N, int G, int nseq, int ragged) {
     c.n = nseq;
     return c;
   }
-  long long n = 4096 / waves;
+  long long n = 3072 / waves;                      // one round of the three waves that fit each of 1024 SIMDs
   if (n < 1) n = 1;
   long long len = (T + n - 1) / n;
-  len = (len + TT - 1) / TT * TT;
+  len = (len + 15) / 16 * 16;
   if (len < 64) len = 64;
   while (T / len >= 65535) len *= 2;               // the chunks are one launch's second dimension
   c.len = (int)len;
@@ -649,19 +737,27 @@ Chunks plan(int T, int D, int N, int G, int nseq, int ragged) {
   return c;
 }
 
-template <int SPL, int LPC, int CPT>
-void launch_scan(const ActhSsmScanDesc& d, const Chunks& ck, int vec, bool chunked, hipStream_t stream) {
+template <int SPL, int LPC, int CPT, bool VEC>
+void launch_scan(const ActhSsmScanDesc& d, const Chunks& ck, bool chunked, hipStream_t stream) {
   constexpr int CB = 64 / LPC * CPT;
   const dim3 grid((unsigned)ck.n, (unsigned)(d.G * ((d.D / d.G + CB - 1) / CB)));
   if (chunked) {
     const long long dn = (long long)d.D * d.N;
-    ssm_scan_kernel<SPL, LPC, CPT, true><<<grid, 64, 0, stream>>>(d, ck, vec);
+    ssm_scan_kernel<SPL, LPC, CPT, true, VEC><<<grid, 64, 0, stream>>>(d, ck);
     ssm_carry_kernel<<<(unsigned)((dn + 255) / 256), 256, 0, stream>>>(d, ck);
-    ssm_scan_kernel<SPL, LPC, CPT, false><<<grid, 64, 0, stream>>>(d, ck, vec);
-    if (d.state) ssm_keep_kernel<<<dim3((unsigned)((dn + 255) / 256), (unsigned)ck.n), 256, 0, stream>>>(d, ck);
+    ssm_scan_kernel<SPL, LPC, CPT, false, VEC><<<grid, 64, 0, stream>>>(d, ck);
+    if (d.state) ssm_keep_kernel<<<dim3((unsigned)((dn + 4095) / 4096), (unsigned)ck.n), 256, 0, stream>>>(d, ck);
   } else {
-    ssm_scan_kernel<SPL, LPC, CPT, false><<<grid, 64, 0, stream>>>(d, ck, vec);
+    ssm_scan_kernel<SPL, LPC, CPT, false, VEC><<<grid, 64, 0, stream>>>(d, ck);
   }
+}
+
+template <bool VEC>
+void launch_scan_n(const ActhSsmScanDesc& d, const Chunks& ck, bool chunked, hipStream_t stream) {
+  if (d.N <= 8) launch_scan<8, 1, 1, VEC>(d, ck, chunked, stream);
+  else if (d.N <= 16) launch_scan<16, 1, 1, VEC>(d, ck, chunked, stream);
+  else if (d.N <= 32) launch_scan<16, 2, 1, VEC>(d, ck, chunked, stream);
+  else launch_scan<16, 4, 1, VEC>(d, ck, chunked, stream);
 }
 
 bool al16(const void* p, long long ld_bytes) { return !p || (((uintptr_t)p | (uintptr_t)ld_bytes) % 16) == 0; }
@@ -740,12 +836,10 @@ extern "C" int acth_ssm_scan(const ActhSsmScanDesc* d, hipStream_t stream) {
     ck.s = d->ws + (size_t)ck.n * d->D * d->N;
   }
   if (d->G * ((d->D / d->G + 15) / 16) > 65535) return ACTH_EINVAL;
-  const int vec = d->D / d->G % 8 == 0 && al16(d->u, d->ldu * 2) && al16(d->delta, d->ld_delta * (d->delta_f32 ? 4 : 2)) &&
+  const bool vec = d->D / d->G % 8 == 0 && al16(d->u, d->ldu * 2) && al16(d->delta, d->ld_delta * (d->delta_f32 ? 4 : 2)) &&
                   al16(d->z, d->ldz * 2) && al16(d->y, d->ldy * 2);
-  if (d->N <= 8) launch_scan<8, 1, 1>(*d, ck, vec, need != 0, stream);
-  else if (d->N <= 16) launch_scan<16, 1, 1>(*d, ck, vec, need != 0, stream);
-  else if (d->N <= 32) launch_scan<16, 2, 1>(*d, ck, vec, need != 0, stream);
-  else launch_scan<16, 4, 1>(*d, ck, vec, need != 0, stream);
+  if (vec) launch_scan_n<true>(*d, ck, need != 0, stream);
+  else launch_scan_n<false>(*d, ck, need != 0, stream);
   ACTH_CHECK_LAUNCH();
   return ACTH_OK;
 }
