@@ -13,7 +13,7 @@
 // of magnitudes: far below a 16-bit output's half step of 2^-9 or 2^-12. fp32 outputs would show it (1.8e-5 of their
 // norm), so those products go through the 16-bit matrix instructions instead, where e4m3 values are exact and the same
 // sums are off by 1e-9 to 1e-8; that unit runs at half the rate.
-#include "common.h"
+#include "gemm_common.h"
 
 namespace {
 
@@ -25,14 +25,14 @@ __device__ __forceinline__ f32x4_t mfma8(i32x8_t a, i32x8_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
 }
 
-__device__ __forceinline__ i32x8_t frag(const uint8_t* lds, int at0, int at1) {
+__device__ __forceinline__ i32x8_t frag(const char* lds, int at0, int at1) {
   const int4 lo = *reinterpret_cast<const int4*>(lds + at0);
   const int4 hi = *reinterpret_cast<const int4*>(lds + at1);
   return (i32x8_t){lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 }
 
 // the 16-bit forms of the 8 bytes at `lds`, exactly
-__device__ __forceinline__ bf16x8_t wide8(const uint8_t* lds) {
+__device__ __forceinline__ bf16x8_t wide8(const char* lds) {
   const int2 v = *reinterpret_cast<const int2*>(lds);
   bf16x8_t o;
 #pragma unroll
@@ -88,7 +88,7 @@ __device__ __forceinline__ int4 load16_any(const uint8_t* p) {
 template <bool WIDE>
 __global__ __launch_bounds__(256) void gemm_fp8_any_kernel(const ActhGemmFp8Desc p, int vec_out) {
   constexpr int PITCH = 144;
-  __shared__ __align__(16) uint8_t sa[64 * PITCH], sw[64 * PITCH];
+  __shared__ __align__(16) char sa[64 * PITCH], sw[64 * PITCH];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int m0 = blockIdx.x * 64, n0 = blockIdx.y * 64;
   const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
@@ -178,6 +178,144 @@ __global__ __launch_bounds__(256) void gemm_fp8_any_kernel(const ActhGemmFp8Desc
     for (int j = 0; j < 2; ++j) finish4(p, m0 + wm + i * 16 + r16, n0 + wn + j * 16 + g * 4, acc[i][j], vec_out);
 }
 
+// ---- large tiles: BM x BN, eight waves of TM x TN fragments, one k block (128 bytes a row) a step, double-buffered
+// LDS-DMA. 16-byte chunk c of row r lies at chunk c ^ (r % 8) of its 128-byte LDS row, so the 8 lanes of a ds_read_b128
+// group, which read one chunk of 8 rows, meet 8 different bank slots; the DMA, whose LDS side is linear, applies the
+// same exchange to its global side.
+template <int BM, int BN>
+struct Tile {
+  static constexpr int WC = BN / 64, WR = 8 / WC;              // waves along n and m
+  static constexpr int TM = BM / WR / 16, TN = 4;              // fragments of a wave
+  static constexpr int AB = BM * 128, STAGE = (BM + BN) * 128;
+  static constexpr int AP = BM / 64, WP = BN / 64;             // DMA pieces of 8 rows a wave and step
+};
+
+}  // namespace
+
+// One step: the DMA of the next k block into `wr`, the products of the block in `rd`. The two stage buffers come in as
+// restricted pointers of their own: told apart, the reads of one need not wait for the loads into the other (the
+// compiler otherwise drains all LDS-DMA before every ds_read).
+template <int BM, int BN>
+struct Stage {
+  using T = Tile<BM, BN>;
+  __amdgpu_buffer_rsrc_t ra, rw, rs;
+  unsigned oa[T::AP], ow[T::WP], os;
+  int wave, chunk, K;
+  long long as_blk;
+
+  __device__ __forceinline__ void dma(char* wr, int kb) const {
+    const bool dead = kb * 128 + chunk * 16 >= K;
+#pragma unroll
+    for (int u = 0; u < T::AP; ++u)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)(wr + (wave + 8 * u) * 1024), 16, dead ? gemm::OOB : oa[u], kb * 128, 0, 0);
+#pragma unroll
+    for (int u = 0; u < T::WP; ++u)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_void*)(wr + T::AB + (wave + 8 * u) * 1024), 16, dead ? gemm::OOB : ow[u], kb * 128, 0, 0);
+    if (wave < BM / 64)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(wr + T::AB + BN * 128 + wave * 256), 4, os, (int)(kb * as_blk * 4), 0, 0);
+  }
+};
+
+template <int BM, int BN>
+__device__ __forceinline__ void step(const char* __restrict__ rd, char* __restrict__ wr, const Stage<BM, BN>& st, int next, bool more,
+                                     int a_row, int w_row, int s_row, int f0, int f1, float ws,
+                                     f32x4_t (&acc)[Tile<BM, BN>::TM][Tile<BM, BN>::TN]) {
+  using T = Tile<BM, BN>;
+  if (more) st.dma(wr, next);
+  i32x8_t fw[T::TN];
+#pragma unroll
+  for (int j = 0; j < T::TN; ++j) fw[j] = frag(rd, w_row + j * 2048 + f0, w_row + j * 2048 + f1);
+  f32x4_t d[2][T::TN];
+  float sc[2];
+#pragma unroll
+  for (int i = 0; i <= T::TM; ++i) {
+    if (i < T::TM) {
+      const i32x8_t fa = frag(rd, a_row + i * 2048 + f0, a_row + i * 2048 + f1);
+      sc[i & 1] = *reinterpret_cast<const float*>(rd + s_row + i * 64) * ws;
+#pragma unroll
+      for (int j = 0; j < T::TN; ++j) d[i & 1][j] = mfma8(fw[j], fa, (f32x4_t){0, 0, 0, 0});
+    }
+    if (i > 0) {
+#pragma unroll
+      for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i - 1][j][e] = fmaf(d[(i - 1) & 1][j][e], sc[(i - 1) & 1], acc[i - 1][j][e]);
+    }
+  }
+}
+
+template <int BM, int BN>
+__global__ __launch_bounds__(512, 2) void gemm_fp8_kernel(const ActhGemmFp8Desc p, int gm, int vec_out) {
+  using T = Tile<BM, BN>;
+  constexpr int STAGE = T::STAGE + BM * 4;                      // a block's rows of A, of W, and the row scales
+  constexpr int MAXKB = 1024;
+  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + MAXKB * (BN / 128) * 4];
+  float* const s_ws = reinterpret_cast<float*>(smem + 2 * STAGE);             // [kb][BN / 128]
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave % T::WR, wc = wave / T::WR;
+  const int r16 = lane & 15, g = lane >> 4;
+
+  // tiles: each XCD takes a contiguous run; inside it gm row blocks x all column blocks, rows fastest
+  const int ntn = (p.N + BN - 1) / BN, ntm = (p.M + BM - 1) / BM, nwg = gridDim.x;
+  const int xcd = blockIdx.x & 7, qn = nwg >> 3, rn = nwg & 7;
+  const int lin = (xcd < rn ? xcd * (qn + 1) : rn * (qn + 1) + (xcd - rn) * qn) + (blockIdx.x >> 3);
+  const int grp = lin / (gm * ntn), mg0 = grp * gm, gcur = min(gm, ntm - mg0), rest = lin - grp * gm * ntn;
+  const int n0 = rest / gcur * BN, m0 = (mg0 + rest % gcur) * BM;
+  const int nkb = (p.K + 127) / 128;
+
+  const int mrows = min(BM, p.M - m0), nrows = min(BN, p.N - n0);
+  Stage<BM, BN> st;
+  st.ra = gemm::make_rsrc((const uint8_t*)p.A + (long long)m0 * p.lda, (unsigned)((mrows - 1) * p.lda + p.K));
+  st.rw = gemm::make_rsrc((const uint8_t*)p.W + (long long)n0 * p.ldw, (unsigned)((nrows - 1) * p.ldw + p.K));
+  st.rs = gemm::make_rsrc(p.ascale + (long long)m0 * p.as_row, 0x7fffffffu);
+  st.wave = wave; st.chunk = (lane & 7) ^ (lane >> 3); st.K = p.K; st.as_blk = p.as_blk;
+#pragma unroll
+  for (int u = 0; u < T::AP; ++u) {
+    const int r = (wave + 8 * u) * 8 + (lane >> 3);
+    st.oa[u] = r < mrows ? (unsigned)(r * p.lda + st.chunk * 16) : gemm::OOB;
+  }
+#pragma unroll
+  for (int u = 0; u < T::WP; ++u) {
+    const int r = (wave + 8 * u) * 8 + (lane >> 3);
+    st.ow[u] = r < nrows ? (unsigned)(r * p.ldw + st.chunk * 16) : gemm::OOB;
+  }
+  st.os = (unsigned)(min(wave * 64 + lane, mrows - 1) * p.as_row * 4);
+
+  f32x4_t acc[T::TM][T::TN];
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < T::TN; ++j) acc[i][j] = (f32x4_t){0, 0, 0, 0};
+
+  st.dma(smem, 0);
+  for (int i = tid; i < nkb * (BN / 128); i += 512) {
+    const int kb = i / (BN / 128), nb = n0 / 128 + i % (BN / 128);
+    s_ws[i] = nb * 128 < p.N ? p.wscale[(long long)nb * p.ws_row + kb * p.ws_blk] : 0.0f;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+
+  const int f0 = (g ^ (r16 & 7)) * 16, f1 = ((g + 4) ^ (r16 & 7)) * 16;
+  const int a_row = (wr * T::TM * 16 + r16) * 128, w_row = T::AB + (wc * 64 + r16) * 128;
+  const int s_row = T::STAGE + (wr * T::TM * 16 + r16) * 4;
+  for (int kb = 0; kb < nkb; ++kb) {
+    const float ws = s_ws[kb * (BN / 128) + wc * 64 / 128];
+    step<BM, BN>(smem + (kb & 1) * STAGE, smem + (~kb & 1) * STAGE, st, kb + 1, kb + 1 < nkb, a_row, w_row, s_row, f0, f1, ws, acc);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < T::TN; ++j)
+      finish4(p, m0 + (wr * T::TM + i) * 16 + r16, n0 + wc * 64 + j * 16 + g * 4, acc[i][j], vec_out);
+}
+
+namespace {
+
 bool al(const void* p, long long ld_bytes, int to) { return !p || (((uintptr_t)p | (uintptr_t)ld_bytes) % to) == 0; }
 
 }  // namespace
@@ -190,6 +328,14 @@ extern "C" int acth_gemm_fp8(const ActhGemmFp8Desc* d, hipStream_t stream) {
     return ACTH_EINVAL;
   const int vec_out = al(d->C, d->ldc * (d->out_f32 ? 4 : 2), 16) && al(d->bias, 0, 16) && al(d->R, d->ldr * 2, 8);
   if (d->N > 65535 * 64) return ACTH_EINVAL;
+  const bool dma = d->K % 16 == 0 && al(d->A, d->lda, 16) && al(d->W, d->ldw, 16) && d->lda < (1 << 22) && d->ldw < (1 << 22) &&
+                   d->K <= 128 * 1024 && 256 * d->as_row < (1 << 28) && (d->K + 127) / 128 * d->as_blk < (1 << 28);
+  if (dma && !d->out_f32 && d->M > 128) {
+    const int ntm = (d->M + 255) / 256, ntn = (d->N + 255) / 256;
+    gemm_fp8_kernel<256, 256><<<(unsigned)(ntm * ntn), 512, 0, stream>>>(*d, 8, vec_out);
+    ACTH_CHECK_LAUNCH();
+    return ACTH_OK;
+  }
   const dim3 grid((unsigned)((d->M + 63) / 64), (unsigned)((d->N + 63) / 64));
   if (d->out_f32) gemm_fp8_any_kernel<true><<<grid, 256, 0, stream>>>(*d, vec_out);
   else gemm_fp8_any_kernel<false><<<grid, 256, 0, stream>>>(*d, vec_out);
