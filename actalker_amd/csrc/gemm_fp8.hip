@@ -31,13 +31,12 @@ __device__ __forceinline__ i32x8_t frag(const char* lds, int at0, int at1) {
   return (i32x8_t){lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 }
 
-// the 16-bit forms of the 8 bytes at `lds`, exactly
-__device__ __forceinline__ bf16x8_t wide8(const char* lds) {
-  const int2 v = *reinterpret_cast<const int2*>(lds);
+// the 16-bit forms of 8 bytes, exactly
+__device__ __forceinline__ bf16x8_t wide8(int x0, int x1) {
   bf16x8_t o;
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    const int x = w ? v.y : v.x;
+    const int x = w ? x1 : x0;
 #if ACTH_F16
     const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false);
     const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true);
@@ -48,6 +47,11 @@ __device__ __forceinline__ bf16x8_t wide8(const char* lds) {
     o[4 * w] = lo[0]; o[4 * w + 1] = lo[1]; o[4 * w + 2] = hi[0]; o[4 * w + 3] = hi[1];
   }
   return o;
+}
+
+__device__ __forceinline__ bf16x8_t wide8(const char* lds) {
+  const int2 v = *reinterpret_cast<const int2*>(lds);
+  return wide8(v.x, v.y);
 }
 
 // bias, residual and store of four consecutive columns [n, n + 4) of row m
@@ -216,36 +220,50 @@ struct Stage {
   }
 };
 
-template <int BM, int BN>
+// Products run LAG ahead of the multiply-adds that take them in, in exactly this order (sched_barrier): the matrix unit
+// then never waits for the vector unit's use of its last result. LAG 1, 2, 3, 4, 8: 571, 546, 531, 528, 528 us at 8192^3.
+constexpr int LAG = 3;
+
+template <int BM, int BN, bool WIDE>
 __device__ __forceinline__ void step(const char* __restrict__ rd, char* __restrict__ wr, const Stage<BM, BN>& st, int next, bool more,
                                      int a_row, int w_row, int s_row, int f0, int f1, float ws,
                                      f32x4_t (&acc)[Tile<BM, BN>::TM][Tile<BM, BN>::TN]) {
   using T = Tile<BM, BN>;
-  if (more) st.dma(wr, next);
-  i32x8_t fw[T::TN];
+  i32x8_t fw[T::TN], fa[2];
+  float sc[T::TM];
+  fa[0] = frag(rd, a_row + f0, a_row + f1);
 #pragma unroll
   for (int j = 0; j < T::TN; ++j) fw[j] = frag(rd, w_row + j * 2048 + f0, w_row + j * 2048 + f1);
-  f32x4_t d[2][T::TN];
-  float sc[2];
 #pragma unroll
-  for (int i = 0; i <= T::TM; ++i) {
-    if (i < T::TM) {
-      const i32x8_t fa = frag(rd, a_row + i * 2048 + f0, a_row + i * 2048 + f1);
-      sc[i & 1] = *reinterpret_cast<const float*>(rd + s_row + i * 64) * ws;
+  for (int i = 0; i < T::TM; ++i) sc[i] = *reinterpret_cast<const float*>(rd + s_row + i * 64) * ws;
+  if (more) st.dma(wr, next);
+  f32x4_t d[LAG + 1];
 #pragma unroll
-      for (int j = 0; j < T::TN; ++j) d[i & 1][j] = mfma8(fw[j], fa, (f32x4_t){0, 0, 0, 0});
+  for (int t = 0; t < T::TM * T::TN + LAG; ++t) {
+    const int i = t / T::TN, j = t % T::TN;
+    if (t < T::TM * T::TN) {
+      if (j == 0 && i + 1 < T::TM) fa[(i + 1) & 1] = frag(rd, a_row + (i + 1) * 2048 + f0, a_row + (i + 1) * 2048 + f1);
+      if constexpr (WIDE) {
+        f32x4_t v = {0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          v = mfma16x16x32(wide8(fw[j][2 * c], fw[j][2 * c + 1]), wide8(fa[i & 1][2 * c], fa[i & 1][2 * c + 1]), v);
+        d[t % (LAG + 1)] = v;
+      } else {
+        d[t % (LAG + 1)] = mfma8(fw[j], fa[i & 1], (f32x4_t){0, 0, 0, 0});
+      }
     }
-    if (i > 0) {
+    if (t >= LAG) {
+      const int u = t - LAG;
 #pragma unroll
-      for (int j = 0; j < T::TN; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i - 1][j][e] = fmaf(d[(i - 1) & 1][j][e], sc[(i - 1) & 1], acc[i - 1][j][e]);
+      for (int e = 0; e < 4; ++e) acc[u / T::TN][u % T::TN][e] = fmaf(d[u % (LAG + 1)][e], sc[u / T::TN], acc[u / T::TN][u % T::TN][e]);
     }
+    if (!WIDE) __builtin_amdgcn_sched_barrier(0);
   }
 }
 
-template <int BM, int BN>
-__global__ __launch_bounds__(512, 2) void gemm_fp8_kernel(const ActhGemmFp8Desc p, int gm, int vec_out) {
+template <int BM, int BN, bool WIDE>
+__global__ __launch_bounds__(512, BM * BN > 128 * 128 ? 2 : 4) void gemm_fp8_kernel(const ActhGemmFp8Desc p, int gm, int vec_out) {
   using T = Tile<BM, BN>;
   constexpr int STAGE = T::STAGE + BM * 4;                      // a block's rows of A, of W, and the row scales
   constexpr int MAXKB = 1024;
@@ -302,7 +320,7 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_kernel(const ActhGemmFp8Desc 
   const int s_row = T::STAGE + (wr * T::TM * 16 + r16) * 4;
   for (int kb = 0; kb < nkb; ++kb) {
     const float ws = s_ws[kb * (BN / 128) + wc * 64 / 128];
-    step<BM, BN>(smem + (kb & 1) * STAGE, smem + (~kb & 1) * STAGE, st, kb + 1, kb + 1 < nkb, a_row, w_row, s_row, f0, f1, ws, acc);
+    step<BM, BN, WIDE>(smem + (kb & 1) * STAGE, smem + (~kb & 1) * STAGE, st, kb + 1, kb + 1 < nkb, a_row, w_row, s_row, f0, f1, ws, acc);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   }
@@ -314,7 +332,133 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_kernel(const ActhGemmFp8Desc 
       finish4(p, m0 + (wr * T::TM + i) * 16 + r16, n0 + wc * 64 + j * 16 + g * 4, acc[i][j], vec_out);
 }
 
+
+template __global__ void gemm_fp8_kernel<256, 256, false>(const ActhGemmFp8Desc, int, int);
+template __global__ void gemm_fp8_kernel<128, 128, false>(const ActhGemmFp8Desc, int, int);
+template __global__ void gemm_fp8_kernel<128, 128, true>(const ActhGemmFp8Desc, int, int);
+
 namespace {
+
+// ---- few rows: a tile of 16 MT x 16 NT, its k blocks dealt to the eight waves in turn (few rows make few tiles, so the
+// long axis has to fill the chip), each wave's fragments straight from memory: no wave waits for another until the
+// partial sums meet in LDS, in a fixed order. A lane loads two 16-byte pieces of its row, k [16 g, 16 g + 16) and 64
+// further. Rows behind the last read it again.
+// Bound: the weights' bytes and the latency of the two or three blocks each wave takes (1 x 10240 x 2560: 8.5 us, 3.1 TB/s;
+// 1 x 2560 x 2560: 5.6 us; two or four blocks' loads at once changed neither), then L2, which serves A and W to every
+// tile: larger row counts take larger tiles.
+template <int MT, int NT, bool WIDE>
+__global__ __launch_bounds__(512, MT * NT > 8 ? 2 : 4) void gemm_fp8_few_kernel(const ActhGemmFp8Desc p, int vec_out) {
+  constexpr int TILES = MT * NT;
+  __shared__ __attribute__((aligned(16))) f32x4_t red[4][TILES][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
+  const int ntm = (p.M + 16 * MT - 1) / (16 * MT);
+  const int m0 = (int)(blockIdx.x % ntm) * 16 * MT, n0 = (int)(blockIdx.x / ntm) * 16 * NT;
+  const int nkb = (p.K + 127) / 128;
+  const int mrows = min(16 * MT, p.M - m0), nrows = min(16 * NT, p.N - n0);
+  const __amdgpu_buffer_rsrc_t ra = gemm::make_rsrc((const uint8_t*)p.A + (long long)m0 * p.lda, (unsigned)((mrows - 1) * p.lda + p.K));
+  const __amdgpu_buffer_rsrc_t rw = gemm::make_rsrc((const uint8_t*)p.W + (long long)n0 * p.ldw, (unsigned)((nrows - 1) * p.ldw + p.K));
+  unsigned oa[MT], ow[NT];
+  const float* as[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int r = min(i * 16 + r16, mrows - 1);
+    oa[i] = (unsigned)(r * p.lda + g * 16);
+    as[i] = p.ascale + (long long)(m0 + r) * p.as_row;
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) ow[j] = (unsigned)(min(j * 16 + r16, nrows - 1) * p.ldw + g * 16);
+  const float* const wsp = p.wscale + (long long)(n0 >> 7) * p.ws_row;       // 16 NT divides 128: one block of columns
+
+  f32x4_t acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4_t){0, 0, 0, 0};
+
+  typedef int i32x4_t __attribute__((ext_vector_type(4)));
+  i32x4_t fa[MT][2], fw[NT][2];
+  for (int kb = wave; kb < nkb; kb += 8) {
+    const int k0 = kb * 128;
+    const bool in0 = k0 + g * 16 < p.K, in1 = k0 + 64 + g * 16 < p.K;      // pieces behind K: zeros
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      fw[j][0] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, in0 ? ow[j] : gemm::OOB, k0, 0));
+      fw[j][1] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, in1 ? ow[j] + 64 : gemm::OOB, k0, 0));
+    }
+    float sc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      fa[i][0] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ra, in0 ? oa[i] : gemm::OOB, k0, 0));
+      fa[i][1] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ra, in1 ? oa[i] + 64 : gemm::OOB, k0, 0));
+      sc[i] = as[i][kb * p.as_blk];
+    }
+    const float ws = wsp[kb * p.ws_blk];
+    f32x4_t d[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) d[i][j] = (f32x4_t){0, 0, 0, 0};
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        bf16x8_t wa[MT], ww[NT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) wa[i] = wide8(fa[i][c >> 1][(c & 1) * 2], fa[i][c >> 1][(c & 1) * 2 + 1]);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) ww[j] = wide8(fw[j][c >> 1][(c & 1) * 2], fw[j][c >> 1][(c & 1) * 2 + 1]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) d[i][j] = mfma16x16x32(ww[j], wa[i], d[i][j]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          d[i][j] = mfma8(__builtin_shufflevector(fw[j][0], fw[j][1], 0, 1, 2, 3, 4, 5, 6, 7),
+                          __builtin_shufflevector(fa[i][0], fa[i][1], 0, 1, 2, 3, 4, 5, 6, 7), d[i][j]);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const float s = sc[i] * ws;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[i][j][e], s, acc[i][j][e]);
+    }
+  }
+
+  // waves 4 .. 7 to 0 .. 3, then every wave sums its share of the tiles over the four
+  if (wave >= 4) {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) red[wave - 4][t][lane] = acc[t / NT][t % NT];
+  }
+  __syncthreads();
+  if (wave < 4) {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) red[wave][t][lane] += acc[t / NT][t % NT];
+  }
+  __syncthreads();
+  for (int t = wave; t < TILES; t += 8) {
+    const f32x4_t v = (red[0][t][lane] + red[1][t][lane]) + (red[2][t][lane] + red[3][t][lane]);
+    finish4(p, m0 + t / NT * 16 + r16, n0 + t % NT * 16 + g * 4, v, vec_out);
+  }
+}
+
+template <bool WIDE>
+void launch_few(const ActhGemmFp8Desc& d, int vec_out, hipStream_t stream) {
+  auto tiles = [&](int mt, int nt) { return (unsigned)(((d.M + 16 * mt - 1) / (16 * mt)) * ((d.N + 16 * nt - 1) / (16 * nt))); };
+  if (d.M <= 16) {
+    if (tiles(1, 4) >= 128) gemm_fp8_few_kernel<1, 4, WIDE><<<tiles(1, 4), 512, 0, stream>>>(d, vec_out);
+    else gemm_fp8_few_kernel<1, 2, WIDE><<<tiles(1, 2), 512, 0, stream>>>(d, vec_out);
+  } else if (d.M <= 32 || tiles(4, 4) < 128) {
+    gemm_fp8_few_kernel<2, 4, WIDE><<<tiles(2, 4), 512, 0, stream>>>(d, vec_out);
+  } else {
+    gemm_fp8_few_kernel<4, 4, WIDE><<<tiles(4, 4), 512, 0, stream>>>(d, vec_out);
+  }
+}
 
 bool al(const void* p, long long ld_bytes, int to) { return !p || (((uintptr_t)p | (uintptr_t)ld_bytes) % to) == 0; }
 
@@ -330,9 +474,23 @@ extern "C" int acth_gemm_fp8(const ActhGemmFp8Desc* d, hipStream_t stream) {
   if (d->N > 65535 * 64) return ACTH_EINVAL;
   const bool dma = d->K % 16 == 0 && al(d->A, d->lda, 16) && al(d->W, d->ldw, 16) && d->lda < (1 << 22) && d->ldw < (1 << 22) &&
                    d->K <= 128 * 1024 && 256 * d->as_row < (1 << 28) && (d->K + 127) / 128 * d->as_blk < (1 << 28);
-  if (dma && !d->out_f32 && d->M > 128) {
-    const int ntm = (d->M + 255) / 256, ntn = (d->N + 255) / 256;
-    gemm_fp8_kernel<256, 256><<<(unsigned)(ntm * ntn), 512, 0, stream>>>(*d, 8, vec_out);
+  if (dma) {
+    const long long t256 = (long long)((d->M + 255) / 256) * ((d->N + 255) / 256);
+    const long long t128 = (long long)((d->M + 127) / 128) * ((d->N + 127) / 128);
+    // Rounds of the chip: 256 large tiles, or 512 small ones (two blocks a CU), in 1.5 times a small round's time
+    // (42 and 27.5 us at K = 2560). 4096 x 2560: 47 against 50 us, 4096 x 5120: 87 against 72, 16384 x 2560: 253 against 276.
+    const long long r256 = (t256 + 255) / 256, r128 = (t128 + 511) / 512;
+    if (d->M <= 32 || t128 <= 40) {              // 256 x 2560 x 2560: 14.6 against 16.2 us, 512 rows: 27.5 against 16.7
+
+      if (d->out_f32) launch_few<true>(*d, vec_out, stream);
+      else launch_few<false>(*d, vec_out, stream);
+    } else if (d->out_f32) {
+      gemm_fp8_kernel<128, 128, true><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
+    } else if (3 * r256 <= 2 * r128) {
+      gemm_fp8_kernel<256, 256, false><<<(unsigned)t256, 512, 0, stream>>>(*d, 8, vec_out);
+    } else {
+      gemm_fp8_kernel<128, 128, false><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
+    }
     ACTH_CHECK_LAUNCH();
     return ACTH_OK;
   }
