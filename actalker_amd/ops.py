@@ -858,37 +858,49 @@ SSM_MAX_STATES = 64
 _CHECK_ARGS = os.environ.get("ACTH_CHECK_ARGS", "0") == "1"
 
 
-def _served(what: str, *tensors) -> torch.device:
-    """The one device of the operands that are given; refuses CPU tensors, several devices and autograd."""
-    dev = tensors[0].device
-    grad = torch.is_grad_enabled()
+def _served(what: str, *tensors) -> int:
+    """Index of the one device of the operands that are given; refuses CPU tensors, several devices and autograd."""
+    idx = tensors[0].get_device()
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise _lib.ActhError(f"{what}: expected a device tensor, got {t.device}")
-        if t.device != dev:
-            raise _lib.ActhError(f"{what}: operands on {dev} and {t.device}")
-        if grad and t.requires_grad:
-            raise _lib.ActhError(f"{what} has no backward: call it under torch.no_grad() or detach its operands")
-    return dev
+        if t is not None and (idx < 0 or t.get_device() != idx):
+            t = tensors[0] if idx < 0 else t
+            if not t.is_cuda:
+                raise _lib.ActhError(f"{what}: expected a device tensor, got {t.device}")
+            raise _lib.ActhError(f"{what}: operands on {tensors[0].device} and {t.device}")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise _lib.ActhError(f"{what} has no backward: call it under torch.no_grad() or detach its operands")
+    return idx
 
 
-def _launch_on(dev: torch.device, fn, d, name: str):
-    if dev.index == torch.cuda.current_device():
-        rc = fn(ctypes.byref(d), torch.cuda.current_stream().cuda_stream)
+# One call of these operators is a few microseconds of GPU time at small sizes, so the host path is kept short: the
+# stream as its raw handle, each operand's checks as few tensor calls as they need.
+def _launch_on(idx: int, fn, d, name: str):
+    if idx == torch._C._cuda_getDevice():
+        rc = fn(ctypes.byref(d), torch._C._cuda_getCurrentRawStream(idx))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(ctypes.byref(d), torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(idx):
+            rc = fn(ctypes.byref(d), torch._C._cuda_getCurrentRawStream(idx))
     if rc:
         _lib.check(rc, name)
 
 
+_SERVE_LIBS = {}
+
+
+def _serve_lib(adt: torch.dtype):
+    lib = _SERVE_LIBS.get(adt)
+    if lib is None:
+        lib = _SERVE_LIBS[adt] = _lib.load(adt)
+    return lib
+
+
 def _mat(t: torch.Tensor, shape, dtype, what: str) -> int:
     """Checks a (rows, columns) operand with contiguous rows; its row stride."""
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise _lib.ActhError(f"{what}: expected {dtype}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape) or (t.stride(1) != 1 and t.shape[1] > 1):
+    if t.shape != shape or (t.stride(1) != 1 and shape[1] > 1):
         raise _lib.ActhError(f"{what}: expected a row-major tensor of shape {tuple(shape)}, got {tuple(t.shape)} "
                              f"strides {t.stride()}")
     return t.stride(0)
@@ -898,7 +910,7 @@ def _vec(t: Optional[torch.Tensor], n: int, what: str):
     """Data pointer of an optional contiguous fp32 vector of n entries."""
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+    if t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous():
         raise _lib.ActhError(f"{what}: expected {n} contiguous fp32 entries, got {tuple(t.shape)} {t.dtype}")
     return t.data_ptr()
 
@@ -929,51 +941,52 @@ def _apart(out: torch.Tensor, other: Optional[torch.Tensor], what: str, same_ok:
 
 
 def _rmsnorm(name, x, gamma, eps, residual, sum_out, out, eight, norm):
-    lib = _lib.load(act_dtype())
-    dev = _served(name, x, gamma, residual, sum_out, out)
+    adt = act_dtype()
+    idx = _served(name, x, gamma, residual, sum_out, out)
     if x.dim() != 2 or x.shape[1] < 1:
         raise _lib.ActhError(f"{name}: expected x of shape (rows, C), got {tuple(x.shape)}")
-    M, C = x.shape
-    d = _lib.RmsNormDesc()
-    d.x, d.ldx = x.data_ptr(), _mat(x, (M, C), act_dtype(), name + " x")
+    shape = x.shape
+    M, C = shape
+    dev = x.device
+    ldx = _mat(x, shape, adt, name + " x")
+    res, ldres, res_f32, ldsum, scale, ld_out = None, 0, 0, 0, None, 0
     if residual is not None:
-        if residual.dtype not in (torch.float32, act_dtype()):
-            raise _lib.ActhError(f"{name} residual: expected torch.float32 or {act_dtype()}, got {residual.dtype}")
-        d.res, d.ldres = residual.data_ptr(), _mat(residual, (M, C), residual.dtype, name + " residual")
-        d.res_f32 = int(residual.dtype == torch.float32)
+        kind = residual.dtype
+        if kind is not torch.float32 and kind is not adt:
+            raise _lib.ActhError(f"{name} residual: expected torch.float32 or {adt}, got {kind}")
+        res, ldres, res_f32 = residual.data_ptr(), _mat(residual, shape, kind, name + " residual"), kind is torch.float32
         if sum_out is None:
-            sum_out = torch.empty((M, C), device=dev, dtype=residual.dtype)
+            sum_out, ldsum = torch.empty(shape, device=dev, dtype=kind), C
         else:
+            ldsum = _mat(sum_out, shape, kind, name + " sum_out")
             _apart(sum_out, x, name + " sum_out", same_ok=True)
             _apart(sum_out, residual, name + " sum_out", same_ok=True)
-        d.sum, d.ldsum = sum_out.data_ptr(), _mat(sum_out, (M, C), residual.dtype, name + " sum_out")
+            _apart(sum_out, gamma, name + " sum_out")
     elif sum_out is not None:
         raise _lib.ActhError(f"{name}: sum_out without a residual")
-    d.gamma, d.eps, d.norm = _vec(gamma, C, name + " gamma"), float(eps), int(norm)
-    scale = None
     if eight:
         # rows start at multiples of 16 bytes and a block's scales lie next to each other, as gemm_fp8 reads them
-        out = torch.empty((M, -(-C // 16) * 16), device=dev, dtype=FP8)[:, :C]
-        kb = -(-C // FP8_BLOCK)
-        scale = torch.empty((kb, M), device=dev, dtype=torch.float32).t()
-        d.y, d.ldy, d.eight = out.data_ptr(), out.stride(0), 1
-        d.scale, d.scale_row, d.scale_blk = scale.data_ptr(), 1, M
+        ld_out = -(-C // 16) * 16
+        out = torch.empty((M, ld_out), device=dev, dtype=FP8)
+        if ld_out != C:
+            out = out[:, :C]
+        scale = torch.empty((-(-C // FP8_BLOCK), M), device=dev, dtype=torch.float32).t()
+    elif out is None:
+        out, ld_out = torch.empty(shape, device=dev, dtype=adt), C
     else:
-        if out is None:
-            out = torch.empty((M, C), device=dev, dtype=act_dtype())
-        else:
-            _apart(out, x, name + " out", same_ok=True)
-            _apart(out, residual, name + " out", same_ok=True)
-            _apart(out, sum_out, name + " out")
-            _apart(out, gamma, name + " out")
-        d.y, d.ldy = out.data_ptr(), _mat(out, (M, C), act_dtype(), name + " out")
-    d.M, d.C = M, C
+        ld_out = _mat(out, shape, adt, name + " out")
+        _apart(out, x, name + " out", same_ok=True)
+        _apart(out, residual, name + " out", same_ok=True)
+        _apart(out, sum_out, name + " out")
+        _apart(out, gamma, name + " out")
+    d = _lib.RmsNormDesc(x.data_ptr(), ldx, res, ldres, res_f32, None if sum_out is None else sum_out.data_ptr(), ldsum,
+                         _vec(gamma, C, name + " gamma"), eps, norm, out.data_ptr(), ld_out, eight,
+                         None if scale is None else scale.data_ptr(), 1, M, M, C)
     if M:
-        _launch_on(dev, lib.acth_rmsnorm, d, "acth_rmsnorm")
-    res = (out, scale) if eight else (out,)
-    if sum_out is not None:
-        res += (sum_out,)
-    return res if len(res) > 1 else out
+        _launch_on(idx, _serve_lib(adt).acth_rmsnorm, d, "acth_rmsnorm")
+    if eight:
+        return (out, scale) if sum_out is None else (out, scale, sum_out)
+    return out if sum_out is None else (out, sum_out)
 
 
 def rmsnorm(x: torch.Tensor, gamma: Optional[torch.Tensor], eps: float = 1e-5, *,
@@ -1024,73 +1037,76 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: t
     (M, ceil(K / 128)) (:func:`rmsnorm_fp8`, :func:`quant_fp8`), w (N, K) with w_scale (ceil(N / 128), ceil(K / 128))
     (:func:`pack_fp8`), scales fp32 with any strides. fp32 accumulation; ``bias`` (N) fp32, ``residual`` (M, N) in the
     activation dtype; out in the activation dtype, or fp32 with ``out_f32``. ``out`` may be the residual."""
-    lib = _lib.load(act_dtype())
-    dev = _served("gemm_fp8", a, a_scale, w, w_scale, bias, residual, out)
+    adt = act_dtype()
+    idx = _served("gemm_fp8", a, a_scale, w, w_scale, bias, residual, out)
     if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1] or w.shape[0] < 1 or w.shape[1] < 1:
         raise _lib.ActhError(f"gemm_fp8: a {tuple(a.shape)} and w {tuple(w.shape)} do not match")
     M, K = a.shape
     N = w.shape[0]
     kb, nb = -(-K // FP8_BLOCK), -(-N // FP8_BLOCK)
-    d = _lib.GemmFp8Desc()
-    d.A, d.lda = a.data_ptr(), _mat(a, (M, K), FP8, "gemm_fp8 a")
-    d.W, d.ldw = w.data_ptr(), _mat(w, (N, K), FP8, "gemm_fp8 w")
     for t, shape, what in ((a_scale, (M, kb), "a_scale"), (w_scale, (nb, kb), "w_scale")):
-        if t.dtype != torch.float32 or tuple(t.shape) != shape:
+        if t.dtype is not torch.float32 or t.shape != shape:
             raise _lib.ActhError(f"gemm_fp8 {what}: expected fp32 of shape {shape}, got {tuple(t.shape)} {t.dtype}")
-    d.ascale, d.as_row, d.as_blk = a_scale.data_ptr(), a_scale.stride(0), a_scale.stride(1)
-    d.wscale, d.ws_row, d.ws_blk = w_scale.data_ptr(), w_scale.stride(0), w_scale.stride(1)
-    d.bias = _vec(bias, N, "gemm_fp8 bias")
-    if residual is not None:
-        d.R, d.ldr = residual.data_ptr(), _mat(residual, (M, N), act_dtype(), "gemm_fp8 residual")
-    kind = torch.float32 if out_f32 else act_dtype()
+    kind = torch.float32 if out_f32 else adt
     if out is None:
-        out = torch.empty((M, N), device=dev, dtype=kind)
+        out = torch.empty((M, N), device=a.device, dtype=kind)
     else:
         for t in (a, a_scale, w, w_scale, bias):
             _apart(out, t, "gemm_fp8 out")
         _apart(out, residual, "gemm_fp8 out", same_ok=True)
-    d.C, d.ldc, d.out_f32 = out.data_ptr(), _mat(out, (M, N), kind, "gemm_fp8 out"), int(out_f32)
-    d.M, d.N, d.K = M, N, K
+    d = _lib.GemmFp8Desc(a.data_ptr(), _mat(a, a.shape, FP8, "gemm_fp8 a"), a_scale.data_ptr(), a_scale.stride(0),
+                         a_scale.stride(1), w.data_ptr(), _mat(w, w.shape, FP8, "gemm_fp8 w"), w_scale.data_ptr(),
+                         w_scale.stride(0), w_scale.stride(1), _vec(bias, N, "gemm_fp8 bias"),
+                         None if residual is None else residual.data_ptr(),
+                         0 if residual is None else _mat(residual, (M, N), adt, "gemm_fp8 residual"),
+                         out.data_ptr(), _mat(out, (M, N), kind, "gemm_fp8 out"), out_f32, M, N, K)
     if M:
-        _launch_on(dev, lib.acth_gemm_fp8, d, "acth_gemm_fp8")
+        _launch_on(idx, _serve_lib(adt).acth_gemm_fp8, d, "acth_gemm_fp8")
     return out
 
 
-def _sequences(name, d, T, nb, starts, slots, fresh, state):
-    """Fills the descriptor's sequence fields (ragged: ``starts``; else nb equal ranges)."""
+def _sequences(name, T, nb, starts, slots, fresh, state):
+    """Checks the sequence operands; (starts, slots, fresh pointers, sequences, slots of the state)."""
     if starts is not None:
-        if starts.dtype != torch.int32 or starts.dim() != 1 or starts.numel() < 2 or not starts.is_contiguous():
+        if starts.dtype is not torch.int32 or starts.dim() != 1 or starts.numel() < 2 or not starts.is_contiguous():
             raise _lib.ActhError(f"{name} starts: expected contiguous int32 row offsets, one more than sequences")
-        d.starts = starts.data_ptr()
         nb = starts.numel() - 1
     elif nb < 1 or T % nb:
         raise _lib.ActhError(f"{name}: {T} rows are not {nb} equal sequences")
-    d.nseq = nb
+    nslots = 0
     if state is not None:
-        d.nslots = state.shape[0]
-        if slots is None and d.nslots < nb:
-            raise _lib.ActhError(f"{name}: {d.nslots} states for {nb} sequences")
-        if d.nslots < 1:
-            raise _lib.ActhError(f"{name}: the state has no slots")
+        nslots = state.shape[0]
+        if nslots < (nb if slots is None else 1):
+            raise _lib.ActhError(f"{name}: {nslots} states for {nb} sequences")
     if slots is not None:
         if state is None:
             raise _lib.ActhError(f"{name}: slots without a state")
-        if slots.dtype != torch.int32 or tuple(slots.shape) != (nb,) or not slots.is_contiguous():
+        if slots.dtype is not torch.int32 or slots.shape != (nb,) or not slots.is_contiguous():
             raise _lib.ActhError(f"{name} slots: expected contiguous int32 of {nb} entries")
-        d.slots = slots.data_ptr()
     if fresh is not None:
-        if fresh.dtype not in (torch.bool, torch.uint8) or tuple(fresh.shape) != (nb,) or not fresh.is_contiguous():
+        if fresh.dtype not in (torch.bool, torch.uint8) or fresh.shape != (nb,) or not fresh.is_contiguous():
             raise _lib.ActhError(f"{name} fresh: expected contiguous bool of {nb} entries")
-        d.fresh = fresh.data_ptr()
     if _CHECK_ARGS:
         if starts is not None:
             s = starts.tolist()
             if s[0] < 0 or s[-1] > T or any(a > b for a, b in zip(s, s[1:])):
                 raise _lib.ActhError(f"{name} starts: offsets must rise from >= 0 to <= {T}")
         if slots is not None:
-            used = [v for v in slots.tolist() if 0 <= v < d.nslots]
+            used = [v for v in slots.tolist() if 0 <= v < nslots]
             if len(set(used)) != len(used):
                 raise _lib.ActhError(f"{name} slots: two sequences share a slot")
+    return (None if starts is None else starts.data_ptr(), None if slots is None else slots.data_ptr(),
+            None if fresh is None else fresh.data_ptr(), nb, nslots)
+
+
+def _state(t: torch.Tensor, rows: int, cols: int, dtype, what: str) -> int:
+    """Checks a (slots, rows, cols) state whose slots are contiguous; its slot stride."""
+    shape = t.shape
+    if t.dtype is not dtype or len(shape) != 3 or shape[1] != rows or shape[2] != cols or \
+            (cols > 1 and t.stride(2) != 1) or (rows > 1 and t.stride(1) != cols):
+        raise _lib.ActhError(f"{what}: expected {dtype} (slots, {rows}, {cols}), got {tuple(shape)} {t.dtype} "
+                             f"strides {t.stride()}")
+    return t.stride(0) if shape[0] > 1 else rows * cols
 
 
 def causal_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, nb: int = 1,
@@ -1107,32 +1123,28 @@ def causal_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] =
     bool: start from zeros whatever the state holds. Rows of padding sequences and rows that no sequence holds are left
     as they were in ``out`` (undefined without one); an empty sequence leaves its state."""
     name = "causal_conv"
-    lib = _lib.load(act_dtype())
-    dev = _served(name, x, w, bias, state, starts, slots, fresh, out)
+    adt = act_dtype()
+    idx = _served(name, x, w, bias, state, starts, slots, fresh, out)
     if x.dim() != 2 or w.dim() != 2 or w.shape[0] != x.shape[1] or x.shape[1] < 1 or not 2 <= w.shape[1] <= 4:
         raise _lib.ActhError(f"{name}: x {tuple(x.shape)} and w {tuple(w.shape)} (2 to 4 taps)")
-    T, D = x.shape
+    shape = x.shape
+    T, D = shape
     W = w.shape[1]
-    d = _lib.CausalConvDesc()
-    d.x, d.ldx = x.data_ptr(), _mat(x, (T, D), act_dtype(), name + " x")
-    d.w, d.bias = _vec(w, D * W, name + " w"), _vec(bias, D, name + " bias")
+    p_starts, p_slots, p_fresh, n, nslots = _sequences(name, T, nb, starts, slots, fresh, state)
+    ld_slot = 0
     if state is not None:
-        if state.dtype != act_dtype() or state.dim() != 3 or tuple(state.shape[1:]) != (W - 1, D) or \
-                not state[:1].is_contiguous():
-            raise _lib.ActhError(f"{name} state: expected {act_dtype()} (slots, {W - 1}, {D}), got {tuple(state.shape)} "
-                                 f"{state.dtype} strides {state.stride()}")
-        d.state, d.ld_slot = state.data_ptr(), max(state.stride(0), (W - 1) * D) if state.shape[0] < 2 else state.stride(0)
-        _apart(state, x, name + " state")
-    _sequences(name, d, T, nb, starts, slots, fresh, state)
+        ld_slot = _state(state, W - 1, D, adt, name + " state")
     if out is None:
-        out = torch.empty((T, D), device=dev, dtype=act_dtype())
+        out = torch.empty(shape, device=x.device, dtype=adt)
     else:
         for t in (x, w, bias, state, starts, slots, fresh):
             _apart(out, t, name + " out")
-    d.y, d.ldy = out.data_ptr(), _mat(out, (T, D), act_dtype(), name + " out")
-    d.T, d.D, d.W, d.silu = T, D, W, int(silu)
+    d = _lib.CausalConvDesc(x.data_ptr(), _mat(x, shape, adt, name + " x"), _vec(w, D * W, name + " w"),
+                            _vec(bias, D, name + " bias"), None if state is None else state.data_ptr(), ld_slot,
+                            p_starts, p_slots, p_fresh, out.data_ptr(), _mat(out, shape, adt, name + " out"),
+                            T, D, W, n, nslots, silu)
     if T:
-        _launch_on(dev, lib.acth_causal_conv, d, "acth_causal_conv")
+        _launch_on(idx, _serve_lib(adt).acth_causal_conv, d, "acth_causal_conv")
     return out
 
 
@@ -1156,54 +1168,49 @@ def ssm_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Ten
 
     Sequences as in :func:`causal_conv`; ``state`` (slots, d, N) fp32 is where each goes on from, updated in place."""
     name = "ssm_scan"
-    lib = _lib.load(act_dtype())
     adt = act_dtype()
-    dev = _served(name, u, delta, A, B, C, D, z, delta_bias, state, starts, slots, fresh, out)
+    idx = _served(name, u, delta, A, B, C, D, z, delta_bias, state, starts, slots, fresh, out)
     if u.dim() != 2 or A.dim() != 2 or B.dim() != 2 or A.shape[0] != u.shape[1] or not 1 <= A.shape[1] <= SSM_MAX_STATES \
             or u.shape[1] < 1:
         raise _lib.ActhError(f"{name}: u {tuple(u.shape)}, A {tuple(A.shape)} (1 to {SSM_MAX_STATES} states), "
                              f"B {tuple(B.shape)}")
-    T, dim = u.shape
+    shape = u.shape
+    T, dim = shape
     N = A.shape[1]
-    G = B.shape[1] // N
-    if G < 1 or B.shape[1] % N or dim % G:
-        raise _lib.ActhError(f"{name}: B's {B.shape[1]} columns are not groups of {N} states that divide {dim} channels")
-    if delta.dtype not in (torch.float32, adt) or B.dtype not in (torch.float32, adt):
-        raise _lib.ActhError(f"{name}: delta {delta.dtype} and B {B.dtype} must be torch.float32 or {adt}")
-    d = _lib.SsmScanDesc()
-    d.u, d.ldu = u.data_ptr(), _mat(u, (T, dim), adt, name + " u")
-    d.delta, d.ld_delta = delta.data_ptr(), _mat(delta, (T, dim), delta.dtype, name + " delta")
-    d.delta_f32 = int(delta.dtype == torch.float32)
-    d.A = _vec(A, dim * N, name + " A")
-    d.B, d.ldb = B.data_ptr(), _mat(B, (T, G * N), B.dtype, name + " B")
-    d.C, d.ldc = C.data_ptr(), _mat(C, (T, G * N), B.dtype, name + " C")
-    d.bc_f32 = int(B.dtype == torch.float32)
-    d.Dskip, d.delta_bias = _vec(D, dim, name + " D"), _vec(delta_bias, dim, name + " delta_bias")
-    if z is not None:
-        d.z, d.ldz = z.data_ptr(), _mat(z, (T, dim), adt, name + " z")
+    GN = B.shape[1]
+    G = GN // N
+    if G < 1 or GN % N or dim % G:
+        raise _lib.ActhError(f"{name}: B's {GN} columns are not groups of {N} states that divide {dim} channels")
+    dk, bk = delta.dtype, B.dtype
+    if (dk is not torch.float32 and dk is not adt) or (bk is not torch.float32 and bk is not adt):
+        raise _lib.ActhError(f"{name}: delta {dk} and B {bk} must be torch.float32 or {adt}")
+    p_starts, p_slots, p_fresh, n, nslots = _sequences(name, T, nb, starts, slots, fresh, state)
+    ld_slot = 0
     if state is not None:
-        if state.dtype != torch.float32 or state.dim() != 3 or tuple(state.shape[1:]) != (dim, N) or \
-                not state[:1].is_contiguous():
-            raise _lib.ActhError(f"{name} state: expected fp32 (slots, {dim}, {N}), got {tuple(state.shape)} "
-                                 f"{state.dtype} strides {state.stride()}")
-        d.state, d.ld_slot = state.data_ptr(), max(state.stride(0), dim * N) if state.shape[0] < 2 else state.stride(0)
-    _sequences(name, d, T, nb, starts, slots, fresh, state)
+        ld_slot = _state(state, dim, N, torch.float32, name + " state")
     if out is None:
-        out = torch.empty((T, dim), device=dev, dtype=adt)
+        out = torch.empty(shape, device=u.device, dtype=adt)
     else:
         for t in (u, delta, A, B, C, D, z, delta_bias, state, starts, slots, fresh):
             _apart(out, t, name + " out")
-    d.y, d.ldy = out.data_ptr(), _mat(out, (T, dim), adt, name + " out")
-    d.T, d.D, d.N, d.G, d.softplus = T, dim, N, G, int(softplus)
-    if T:
-        ws = None
-        need = 0 if starts is None and d.nseq == T else \
-            lib.acth_ssm_scan_workspace_size(T, dim, N, G, d.nseq, int(starts is not None))
+    lib = _serve_lib(adt)
+    ws, need = None, 0
+    if T and (starts is not None or n != T):
+        need = lib.acth_ssm_scan_workspace_size(T, dim, N, G, n, starts is not None)
         if need:
-            ws = torch.empty(need // 4, device=dev, dtype=torch.float32)
-            d.ws, d.ws_bytes = ws.data_ptr(), need
-        _launch_on(dev, lib.acth_ssm_scan, d, "acth_ssm_scan")
-        del ws
+            ws = torch.empty(need // 4, device=u.device, dtype=torch.float32)
+    d = _lib.SsmScanDesc(u.data_ptr(), _mat(u, shape, adt, name + " u"),
+                         delta.data_ptr(), _mat(delta, shape, dk, name + " delta"), dk is torch.float32,
+                         _vec(A, dim * N, name + " A"),
+                         B.data_ptr(), _mat(B, (T, GN), bk, name + " B"), C.data_ptr(), _mat(C, (T, GN), bk, name + " C"),
+                         bk is torch.float32, _vec(D, dim, name + " D"), _vec(delta_bias, dim, name + " delta_bias"),
+                         None if z is None else z.data_ptr(), 0 if z is None else _mat(z, shape, adt, name + " z"),
+                         None if state is None else state.data_ptr(), ld_slot, p_starts, p_slots, p_fresh,
+                         out.data_ptr(), _mat(out, shape, adt, name + " out"),
+                         T, dim, N, G, n, nslots, softplus, None if ws is None else ws.data_ptr(), need)
+    if T:
+        _launch_on(idx, lib.acth_ssm_scan, d, "acth_ssm_scan")
+    del ws
     return out
 
 
