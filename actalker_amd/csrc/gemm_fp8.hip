@@ -49,11 +49,6 @@ __device__ __forceinline__ bf16x8_t wide8(int x0, int x1) {
   return o;
 }
 
-__device__ __forceinline__ bf16x8_t wide8(const char* lds) {
-  const int2 v = *reinterpret_cast<const int2*>(lds);
-  return wide8(v.x, v.y);
-}
-
 // bias, residual and store of four consecutive columns [n, n + 4) of row m
 __device__ __forceinline__ void finish4(const ActhGemmFp8Desc& p, int m, int n, f32x4_t v, int vec) {
   if (m >= p.M) return;
@@ -81,105 +76,35 @@ __device__ __forceinline__ void finish4(const ActhGemmFp8Desc& p, int m, int n, 
   }
 }
 
-// 16 bytes from any address: one unaligned load
-__device__ __forceinline__ int4 load16_any(const uint8_t* p) {
+__device__ __forceinline__ int4 load16_whole(const uint8_t* p) {
   struct __attribute__((packed, aligned(1))) Any { int v[4]; };
   const Any a = *reinterpret_cast<const Any*>(p);
   return make_int4(a.v[0], a.v[1], a.v[2], a.v[3]);
 }
 
-// ---- any sizes, strides and alignment: a 64 x 64 tile, four waves of 32 x 32, one k block at a time through LDS
-template <bool WIDE>
-__global__ __launch_bounds__(256) void gemm_fp8_any_kernel(const ActhGemmFp8Desc p, int vec_out) {
-  constexpr int PITCH = 144;
-  __shared__ __align__(16) char sa[64 * PITCH], sw[64 * PITCH];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int m0 = blockIdx.x * 64, n0 = blockIdx.y * 64;
-  const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
-  const int r16 = lane & 15, g = lane >> 4;
-  f32x4_t acc[2][2];
+// bytes [k, k + 16) of a row of K bytes at any address, zeros behind its end: one unaligned load. A piece that the end
+// cuts is loaded from 16 bytes before the end and moved down, so nothing behind the row is read.
+__device__ __forceinline__ int4 load16_any(const uint8_t* row, int k, int K) {
+  struct __attribute__((packed, aligned(1))) Any { unsigned long long v[2]; };
+  if (k >= K) return make_int4(0, 0, 0, 0);
+  unsigned long long lo = 0, hi = 0;
+  if (k + 16 <= K) {
+    const Any a = *reinterpret_cast<const Any*>(row + k);
+    lo = a.v[0]; hi = a.v[1];
+  } else if (K >= 16) {
+    const Any a = *reinterpret_cast<const Any*>(row + K - 16);
+    const int s = (16 - (K - k)) * 8;              // 8 .. 120 bits
+    lo = s < 64 ? (a.v[0] >> s) | (a.v[1] << (64 - s)) : a.v[1] >> (s - 64);
+    hi = s < 64 ? a.v[1] >> s : 0;
+  } else {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = (f32x4_t){0, 0, 0, 0};
-
-  const int nkb = (p.K + 127) / 128;
-  for (int kb = 0; kb < nkb; ++kb) {
-    const int k0 = kb * 128;
-    // 64 rows x 8 pieces of 16 bytes for each operand
-    for (int i = tid; i < 512; i += 256) {
-      const int r = i >> 3, c = (i & 7) * 16;
-#pragma unroll
-      for (int o = 0; o < 2; ++o) {
-        const int row = (o ? n0 : m0) + r, rows = o ? p.N : p.M;
-        const uint8_t* src = o ? (const uint8_t*)p.W + row * p.ldw : (const uint8_t*)p.A + row * p.lda;
-        int4 v = make_int4(0, 0, 0, 0);
-        if (row < rows && k0 + c < p.K) {
-          if (k0 + c + 16 <= p.K) {
-            v = load16_any(src + k0 + c);
-          } else {
-            uint32_t b[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (k0 + c + e < p.K) b[e >> 2] |= (uint32_t)src[k0 + c + e] << (8 * (e & 3));
-            v = make_int4((int)b[0], (int)b[1], (int)b[2], (int)b[3]);
-          }
-        }
-        *reinterpret_cast<int4*>((o ? sw : sa) + r * PITCH + c) = v;
+    for (int e = 0; e < 15; ++e)
+      if (k + e < K) {
+        if (e < 8) lo |= (unsigned long long)row[k + e] << (8 * (e & 7));
+        else hi |= (unsigned long long)row[k + e] << (8 * (e & 7));
       }
-    }
-    __syncthreads();
-    const float ws = p.wscale[(long long)(n0 >> 7) * p.ws_row + kb * p.ws_blk];
-    float sc[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int ra = m0 + wm + i * 16 + r16;
-      sc[i] = ra < p.M ? p.ascale[(long long)ra * p.as_row + kb * p.as_blk] * ws : 0.0f;
-    }
-    f32x4_t d[2][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) d[i][j] = (f32x4_t){0, 0, 0, 0};
-    if constexpr (WIDE) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        bf16x8_t fa[2], fw[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          fa[i] = wide8(sa + (wm + i * 16 + r16) * PITCH + c * 32 + g * 8);
-          fw[i] = wide8(sw + (wn + i * 16 + r16) * PITCH + c * 32 + g * 8);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) d[i][j] = mfma16x16x32(fw[j], fa[i], d[i][j]);
-      }
-    } else {
-      i32x8_t fa[2], fw[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int ra = (wm + i * 16 + r16) * PITCH, rw = (wn + i * 16 + r16) * PITCH;
-        fa[i] = frag(sa, ra + g * 32, ra + g * 32 + 16);
-        fw[i] = frag(sw, rw + g * 32, rw + g * 32 + 16);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) d[i][j] = mfma8(fw[j], fa[i], d[i][j]);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[i][j][e], sc[i], acc[i][j][e]);
-    __syncthreads();
   }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) finish4(p, m0 + wm + i * 16 + r16, n0 + wn + j * 16 + g * 4, acc[i][j], vec_out);
+  return make_int4((int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32));
 }
 
 // ---- large tiles: BM x BN, eight waves of TM x TN fragments, one k block (128 bytes a row) a step, double-buffered
@@ -219,6 +144,18 @@ struct Stage {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(wr + T::AB + BN * 128 + wave * 256), 4, os, (int)(kb * as_blk * 4), 0, 0);
   }
 };
+
+// tiles: each XCD takes a contiguous run; inside it gm row blocks x all column blocks, rows fastest, so the tiles that an
+// XCD holds at once share their rows of A and W in its L2
+template <int BM, int BN>
+__device__ __forceinline__ void tile_of(const ActhGemmFp8Desc& p, int gm, int& m0, int& n0) {
+  const int ntn = (p.N + BN - 1) / BN, ntm = (p.M + BM - 1) / BM, nwg = gridDim.x;
+  const int xcd = blockIdx.x & 7, qn = nwg >> 3, rn = nwg & 7;
+  const int lin = (xcd < rn ? xcd * (qn + 1) : rn * (qn + 1) + (xcd - rn) * qn) + (blockIdx.x >> 3);
+  const int grp = lin / (gm * ntn), mg0 = grp * gm, gcur = min(gm, ntm - mg0), rest = lin - grp * gm * ntn;
+  n0 = rest / gcur * BN;
+  m0 = (mg0 + rest % gcur) * BM;
+}
 
 // Products run LAG ahead of the multiply-adds that take them in, in exactly this order (sched_barrier): the matrix unit
 // then never waits for the vector unit's use of its last result. LAG 1, 2, 3, 4, 8: 571, 546, 531, 528, 528 us at 8192^3.
@@ -263,7 +200,7 @@ __device__ __forceinline__ void step(const char* __restrict__ rd, char* __restri
 }
 
 template <int BM, int BN, bool WIDE>
-__global__ __launch_bounds__(512, BM * BN > 128 * 128 ? 2 : 4) void gemm_fp8_kernel(const ActhGemmFp8Desc p, int gm, int vec_out) {
+__global__ __launch_bounds__(512, BM * BN > 128 * 128 || WIDE ? 2 : 4) void gemm_fp8_kernel(const ActhGemmFp8Desc p, int gm, int vec_out) {
   using T = Tile<BM, BN>;
   constexpr int STAGE = T::STAGE + BM * 4;                      // a block's rows of A, of W, and the row scales
   constexpr int MAXKB = 1024;
@@ -275,12 +212,8 @@ __global__ __launch_bounds__(512, BM * BN > 128 * 128 ? 2 : 4) void gemm_fp8_ker
   const int wr = wave % T::WR, wc = wave / T::WR;
   const int r16 = lane & 15, g = lane >> 4;
 
-  // tiles: each XCD takes a contiguous run; inside it gm row blocks x all column blocks, rows fastest
-  const int ntn = (p.N + BN - 1) / BN, ntm = (p.M + BM - 1) / BM, nwg = gridDim.x;
-  const int xcd = blockIdx.x & 7, qn = nwg >> 3, rn = nwg & 7;
-  const int lin = (xcd < rn ? xcd * (qn + 1) : rn * (qn + 1) + (xcd - rn) * qn) + (blockIdx.x >> 3);
-  const int grp = lin / (gm * ntn), mg0 = grp * gm, gcur = min(gm, ntm - mg0), rest = lin - grp * gm * ntn;
-  const int n0 = rest / gcur * BN, m0 = (mg0 + rest % gcur) * BM;
+  int m0, n0;
+  tile_of<BM, BN>(p, gm, m0, n0);
   const int nkb = (p.K + 127) / 128;
 
   const int mrows = min(BM, p.M - m0), nrows = min(BN, p.N - n0);
@@ -333,9 +266,90 @@ __global__ __launch_bounds__(512, BM * BN > 128 * 128 ? 2 : 4) void gemm_fp8_ker
 }
 
 
+// The 128 x 128 tile for operands that the LDS-DMA cannot take (rows at any address, a K that ends inside 16 bytes, very
+// long rows): the next block goes through registers, loaded before this one's products and written to LDS after them.
+// One block a CU: held to the 128 registers of two it spills (4096 x 2560 x 2561: 118 against 98 us; fp32 outputs of the
+// DMA tile likewise, 4096 x 2560 x 2560: 127 against 78 us).
+template <bool WIDE>
+__global__ __launch_bounds__(512, 2) void gemm_fp8_any_kernel(const ActhGemmFp8Desc p, int gm, int vec_out) {
+  constexpr int BM = 128, BN = 128;
+  using T = Tile<BM, BN>;
+  constexpr int STAGE = T::STAGE + BM * 4;
+  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave % T::WR, wc = wave / T::WR;
+  const int r16 = lane & 15, g = lane >> 4;
+  int m0, n0;
+  tile_of<BM, BN>(p, gm, m0, n0);
+  const int nkb = (p.K + 127) / 128;
+  const int chunk = (lane & 7) ^ (lane >> 3);
+  const uint8_t* ar[T::AP];
+  const uint8_t* wrow[T::WP];
+#pragma unroll
+  for (int u = 0; u < T::AP; ++u) ar[u] = (const uint8_t*)p.A + min(m0 + (wave + 8 * u) * 8 + (lane >> 3), p.M - 1) * p.lda;
+#pragma unroll
+  for (int u = 0; u < T::WP; ++u) wrow[u] = (const uint8_t*)p.W + min(n0 + (wave + 8 * u) * 8 + (lane >> 3), p.N - 1) * p.ldw;
+  const float* const as = p.ascale + min(m0 + tid % BM, p.M - 1) * p.as_row;
+  const float* const ws = p.wscale + (long long)(n0 >> 7) * p.ws_row;
+  int4 ra[T::AP], rw[T::WP];
+  float rs = 0.0f;
+  auto load = [&](int kb) {
+    const int k = kb * 128 + chunk * 16;
+    if (kb * 128 + 128 <= p.K) {                   // a whole block
+#pragma unroll
+      for (int u = 0; u < T::AP; ++u) ra[u] = load16_whole(ar[u] + k);
+#pragma unroll
+      for (int u = 0; u < T::WP; ++u) rw[u] = load16_whole(wrow[u] + k);
+    } else {
+#pragma unroll
+      for (int u = 0; u < T::AP; ++u) ra[u] = load16_any(ar[u], k, p.K);
+#pragma unroll
+      for (int u = 0; u < T::WP; ++u) rw[u] = load16_any(wrow[u], k, p.K);
+    }
+    rs = as[kb * p.as_blk];
+  };
+  auto store = [&](char* to) {
+#pragma unroll
+    for (int u = 0; u < T::AP; ++u) *reinterpret_cast<int4*>(to + (wave + 8 * u) * 1024 + lane * 16) = ra[u];
+#pragma unroll
+    for (int u = 0; u < T::WP; ++u) *reinterpret_cast<int4*>(to + T::AB + (wave + 8 * u) * 1024 + lane * 16) = rw[u];
+    if (tid < BM) *reinterpret_cast<float*>(to + T::STAGE + tid * 4) = rs;
+  };
+
+  f32x4_t acc[T::TM][T::TN];
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < T::TN; ++j) acc[i][j] = (f32x4_t){0, 0, 0, 0};
+
+  load(0);
+  store(smem);
+  __syncthreads();
+  const int f0 = (g ^ (r16 & 7)) * 16, f1 = ((g + 4) ^ (r16 & 7)) * 16;
+  const int a_row = (wr * T::TM * 16 + r16) * 128, w_row = T::AB + (wc * 64 + r16) * 128;
+  const int s_row = T::STAGE + (wr * T::TM * 16 + r16) * 4;
+  const Stage<BM, BN> none = {};
+  for (int kb = 0; kb < nkb; ++kb) {
+    const bool more = kb + 1 < nkb;
+    if (more) load(kb + 1);
+    step<BM, BN, WIDE>(smem + (kb & 1) * STAGE, nullptr, none, 0, false, a_row, w_row, s_row, f0, f1, ws[kb * p.ws_blk], acc);
+    if (more) store(smem + (~kb & 1) * STAGE);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < T::TN; ++j)
+      finish4(p, m0 + (wr * T::TM + i) * 16 + r16, n0 + wc * 64 + j * 16 + g * 4, acc[i][j], vec_out);
+}
+
 template __global__ void gemm_fp8_kernel<256, 256, false>(const ActhGemmFp8Desc, int, int);
 template __global__ void gemm_fp8_kernel<128, 128, false>(const ActhGemmFp8Desc, int, int);
 template __global__ void gemm_fp8_kernel<128, 128, true>(const ActhGemmFp8Desc, int, int);
+template __global__ void gemm_fp8_any_kernel<false>(const ActhGemmFp8Desc, int, int);
+template __global__ void gemm_fp8_any_kernel<true>(const ActhGemmFp8Desc, int, int);
 
 namespace {
 
@@ -346,8 +360,8 @@ namespace {
 // Bound: the weights' bytes and the latency of the two or three blocks each wave takes (1 x 10240 x 2560: 8.5 us, 3.1 TB/s;
 // 1 x 2560 x 2560: 5.6 us; two or four blocks' loads at once changed neither), then L2, which serves A and W to every
 // tile: larger row counts take larger tiles.
-template <int MT, int NT, bool WIDE>
-__global__ __launch_bounds__(512, MT * NT > 8 ? 2 : 4) void gemm_fp8_few_kernel(const ActhGemmFp8Desc p, int vec_out) {
+template <int MT, int NT, bool WIDE, bool ALIGNED>
+__global__ __launch_bounds__(512, MT * NT > 8 || (MT * NT == 8 && (WIDE || !ALIGNED)) ? 2 : 4) void gemm_fp8_few_kernel(const ActhGemmFp8Desc p, int vec_out) {
   constexpr int TILES = MT * NT;
   __shared__ __attribute__((aligned(16))) f32x4_t red[4][TILES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -358,16 +372,22 @@ __global__ __launch_bounds__(512, MT * NT > 8 ? 2 : 4) void gemm_fp8_few_kernel(
   const int mrows = min(16 * MT, p.M - m0), nrows = min(16 * NT, p.N - n0);
   const __amdgpu_buffer_rsrc_t ra = gemm::make_rsrc((const uint8_t*)p.A + (long long)m0 * p.lda, (unsigned)((mrows - 1) * p.lda + p.K));
   const __amdgpu_buffer_rsrc_t rw = gemm::make_rsrc((const uint8_t*)p.W + (long long)n0 * p.ldw, (unsigned)((nrows - 1) * p.ldw + p.K));
-  unsigned oa[MT], ow[NT];
+  unsigned oa[MT], ow[NT];                         // ALIGNED: offsets in the buffers above; else row pointers
+  const uint8_t *pa[MT], *pw[NT];
   const float* as[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int r = min(i * 16 + r16, mrows - 1);
     oa[i] = (unsigned)(r * p.lda + g * 16);
+    pa[i] = (const uint8_t*)p.A + (long long)(m0 + r) * p.lda;
     as[i] = p.ascale + (long long)(m0 + r) * p.as_row;
   }
 #pragma unroll
-  for (int j = 0; j < NT; ++j) ow[j] = (unsigned)(min(j * 16 + r16, nrows - 1) * p.ldw + g * 16);
+  for (int j = 0; j < NT; ++j) {
+    const int r = min(j * 16 + r16, nrows - 1);
+    ow[j] = (unsigned)(r * p.ldw + g * 16);
+    pw[j] = (const uint8_t*)p.W + (long long)(n0 + r) * p.ldw;
+  }
   const float* const wsp = p.wscale + (long long)(n0 >> 7) * p.ws_row;       // 16 NT divides 128: one block of columns
 
   f32x4_t acc[MT][NT];
@@ -383,14 +403,24 @@ __global__ __launch_bounds__(512, MT * NT > 8 ? 2 : 4) void gemm_fp8_few_kernel(
     const bool in0 = k0 + g * 16 < p.K, in1 = k0 + 64 + g * 16 < p.K;      // pieces behind K: zeros
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      fw[j][0] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, in0 ? ow[j] : gemm::OOB, k0, 0));
-      fw[j][1] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, in1 ? ow[j] + 64 : gemm::OOB, k0, 0));
+      if constexpr (ALIGNED) {
+        fw[j][0] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, in0 ? ow[j] : gemm::OOB, k0, 0));
+        fw[j][1] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, in1 ? ow[j] + 64 : gemm::OOB, k0, 0));
+      } else {
+        fw[j][0] = __builtin_bit_cast(i32x4_t, load16_any(pw[j], k0 + g * 16, p.K));
+        fw[j][1] = __builtin_bit_cast(i32x4_t, load16_any(pw[j], k0 + 64 + g * 16, p.K));
+      }
     }
     float sc[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      fa[i][0] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ra, in0 ? oa[i] : gemm::OOB, k0, 0));
-      fa[i][1] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ra, in1 ? oa[i] + 64 : gemm::OOB, k0, 0));
+      if constexpr (ALIGNED) {
+        fa[i][0] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ra, in0 ? oa[i] : gemm::OOB, k0, 0));
+        fa[i][1] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ra, in1 ? oa[i] + 64 : gemm::OOB, k0, 0));
+      } else {
+        fa[i][0] = __builtin_bit_cast(i32x4_t, load16_any(pa[i], k0 + g * 16, p.K));
+        fa[i][1] = __builtin_bit_cast(i32x4_t, load16_any(pa[i], k0 + 64 + g * 16, p.K));
+      }
       sc[i] = as[i][kb * p.as_blk];
     }
     const float ws = wsp[kb * p.ws_blk];
@@ -447,16 +477,16 @@ __global__ __launch_bounds__(512, MT * NT > 8 ? 2 : 4) void gemm_fp8_few_kernel(
   }
 }
 
-template <bool WIDE>
+template <bool WIDE, bool ALIGNED>
 void launch_few(const ActhGemmFp8Desc& d, int vec_out, hipStream_t stream) {
   auto tiles = [&](int mt, int nt) { return (unsigned)(((d.M + 16 * mt - 1) / (16 * mt)) * ((d.N + 16 * nt - 1) / (16 * nt))); };
   if (d.M <= 16) {
-    if (tiles(1, 4) >= 128) gemm_fp8_few_kernel<1, 4, WIDE><<<tiles(1, 4), 512, 0, stream>>>(d, vec_out);
-    else gemm_fp8_few_kernel<1, 2, WIDE><<<tiles(1, 2), 512, 0, stream>>>(d, vec_out);
+    if (tiles(1, 4) >= 128) gemm_fp8_few_kernel<1, 4, WIDE, ALIGNED><<<tiles(1, 4), 512, 0, stream>>>(d, vec_out);
+    else gemm_fp8_few_kernel<1, 2, WIDE, ALIGNED><<<tiles(1, 2), 512, 0, stream>>>(d, vec_out);
   } else if (d.M <= 32 || tiles(4, 4) < 128) {
-    gemm_fp8_few_kernel<2, 4, WIDE><<<tiles(2, 4), 512, 0, stream>>>(d, vec_out);
+    gemm_fp8_few_kernel<2, 4, WIDE, ALIGNED><<<tiles(2, 4), 512, 0, stream>>>(d, vec_out);
   } else {
-    gemm_fp8_few_kernel<4, 4, WIDE><<<tiles(4, 4), 512, 0, stream>>>(d, vec_out);
+    gemm_fp8_few_kernel<4, 4, WIDE, ALIGNED><<<tiles(4, 4), 512, 0, stream>>>(d, vec_out);
   }
 }
 
@@ -471,32 +501,28 @@ extern "C" int acth_gemm_fp8(const ActhGemmFp8Desc* d, hipStream_t stream) {
   if ((d->M > 1 && (d->lda < d->K || d->ldc < d->N || (d->R && d->ldr < d->N))) || (d->N > 1 && d->ldw < d->K))
     return ACTH_EINVAL;
   const int vec_out = al(d->C, d->ldc * (d->out_f32 ? 4 : 2), 16) && al(d->bias, 0, 16) && al(d->R, d->ldr * 2, 8);
-  if (d->N > 65535 * 64) return ACTH_EINVAL;
   const bool dma = d->K % 16 == 0 && al(d->A, d->lda, 16) && al(d->W, d->ldw, 16) && d->lda < (1 << 22) && d->ldw < (1 << 22) &&
                    d->K <= 128 * 1024 && 256 * d->as_row < (1 << 28) && (d->K + 127) / 128 * d->as_blk < (1 << 28);
-  if (dma) {
-    const long long t256 = (long long)((d->M + 255) / 256) * ((d->N + 255) / 256);
-    const long long t128 = (long long)((d->M + 127) / 128) * ((d->N + 127) / 128);
-    // Rounds of the chip: 256 large tiles, or 512 small ones (two blocks a CU), in 1.5 times a small round's time
-    // (42 and 27.5 us at K = 2560). 4096 x 2560: 47 against 50 us, 4096 x 5120: 87 against 72, 16384 x 2560: 253 against 276.
-    const long long r256 = (t256 + 255) / 256, r128 = (t128 + 511) / 512;
-    if (d->M <= 32 || t128 <= 40) {              // 256 x 2560 x 2560: 14.6 against 16.2 us, 512 rows: 27.5 against 16.7
-
-      if (d->out_f32) launch_few<true>(*d, vec_out, stream);
-      else launch_few<false>(*d, vec_out, stream);
-    } else if (d->out_f32) {
-      gemm_fp8_kernel<128, 128, true><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
-    } else if (3 * r256 <= 2 * r128) {
-      gemm_fp8_kernel<256, 256, false><<<(unsigned)t256, 512, 0, stream>>>(*d, 8, vec_out);
-    } else {
-      gemm_fp8_kernel<128, 128, false><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
-    }
-    ACTH_CHECK_LAUNCH();
-    return ACTH_OK;
+  const long long t256 = (long long)((d->M + 255) / 256) * ((d->N + 255) / 256);
+  const long long t128 = (long long)((d->M + 127) / 128) * ((d->N + 127) / 128);
+  if (((long long)d->M + 15) / 16 * (((long long)d->N + 31) / 32) > 0x7fffffff && (d->M <= 32 || t128 <= 40)) return ACTH_EINVAL;
+  if (t128 > 0x7fffffff) return ACTH_EINVAL;
+  // Rounds of the chip: 256 large tiles, or 512 small ones (two blocks a CU), in 1.5 times a small round's time
+  // (42 and 27.5 us at K = 2560). 4096 x 2560: 47 against 50 us, 4096 x 5120: 87 against 72, 16384 x 2560: 253 against 276.
+  const long long r256 = (t256 + 255) / 256, r128 = (t128 + 511) / 512;
+  if (d->M <= 32 || t128 <= 40) {                // 256 x 2560 x 2560: 14.6 against 16.2 us, 512 rows: 27.5 against 16.7
+    if (dma) d->out_f32 ? launch_few<true, true>(*d, vec_out, stream) : launch_few<false, true>(*d, vec_out, stream);
+    else d->out_f32 ? launch_few<true, false>(*d, vec_out, stream) : launch_few<false, false>(*d, vec_out, stream);
+  } else if (!dma) {
+    if (d->out_f32) gemm_fp8_any_kernel<true><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
+    else gemm_fp8_any_kernel<false><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
+  } else if (d->out_f32) {
+    gemm_fp8_kernel<128, 128, true><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
+  } else if (3 * r256 <= 2 * r128) {
+    gemm_fp8_kernel<256, 256, false><<<(unsigned)t256, 512, 0, stream>>>(*d, 8, vec_out);
+  } else {
+    gemm_fp8_kernel<128, 128, false><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
   }
-  const dim3 grid((unsigned)((d->M + 63) / 64), (unsigned)((d->N + 63) / 64));
-  if (d->out_f32) gemm_fp8_any_kernel<true><<<grid, 256, 0, stream>>>(*d, vec_out);
-  else gemm_fp8_any_kernel<false><<<grid, 256, 0, stream>>>(*d, vec_out);
   ACTH_CHECK_LAUNCH();
   return ACTH_OK;
 }

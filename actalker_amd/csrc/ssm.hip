@@ -7,6 +7,8 @@
 // Sequences are row ranges [starts[i], starts[i+1]) of one token-major tensor; `starts` lives on the device, so the
 // host never learns the lengths. Everything read from it is clamped to [0, T], and a slot outside [0, nslots) marks a
 // padding sequence whose rows are left alone, so no content of either can lead an access out of its tensor.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -216,42 +218,59 @@ __global__ __launch_bounds__(64) void causal_conv_kernel(const ActhCausalConvDes
   }
 }
 
-// one row a sequence: a lane takes VEC channels of one sequence. Bound: the kept inputs' bytes; few rows: the launch.
-template <int VEC, int W>
+constexpr int CSTEP = 4;                           // 512 sequences x 5120 channels: 1: 24 us, 4: 17, 8: 15
+
+// One row a sequence: a lane takes VEC channels of SEQS sequences, whose loads are all under way before the first is
+// used, so that the weights are read once for them. Bound: the kept inputs' bytes; few rows: the launch.
+template <int VEC, int W, int SEQS>
 __global__ __launch_bounds__(256) void causal_conv_step_kernel(const ActhCausalConvDesc p) {
-  const int nch = (p.D + VEC - 1) / VEC;
-  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long r = at / nch;
-  const int d = (int)(at - r * nch) * VEC;
-  if (r >= p.T) return;
-  const Seq q = seq_of(p, (int)r);
-  if (p.slots && q.slot < 0) return;
-  ConvLane<VEC, W> c;
-  float win[W - 1][VEC], xv[VEC], yv[VEC];
-  load_c<VEC>((const bf16_t*)p.x + r * p.ldx + d, xv);
-  bf16_t* st = (bf16_t*)p.state + (long long)(q.slot < 0 ? 0 : q.slot) * p.ld_slot + d;
-  const bool kept = seq_kept(p, q);
+  const int d = (blockIdx.x * 256 + threadIdx.x) * VEC;
+  if (d >= p.D) return;
+  const int r0 = blockIdx.y * SEQS;
+  typedef typename std::conditional<VEC == 8, uint4, bf16_t>::type raw_t;
+  raw_t xr[SEQS], wr[SEQS][W - 1];
+  int slot[SEQS];
+  bool kept[SEQS], live[SEQS];
 #pragma unroll
-  for (int j = 0; j < W - 1; ++j) {
+  for (int k = 0; k < SEQS; ++k) {
+    const int r = min(r0 + k, p.T - 1);
+    const Seq q = seq_of(p, r);
+    live[k] = r0 + k < p.T && (!p.slots || q.slot >= 0);
+    slot[k] = q.slot;
+    kept[k] = seq_kept(p, q);
+    xr[k] = *reinterpret_cast<const raw_t*>((const bf16_t*)p.x + (long long)r * p.ldx + d);
+    const bf16_t* st = (const bf16_t*)p.state + (q.slot < 0 ? 0 : q.slot) * p.ld_slot + d;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) win[j][v] = 0.0f;
-    if (kept) load_c<VEC>(st + (long long)j * p.D, win[j]);
+    for (int j = 0; j < W - 1; ++j) {
+      wr[k][j] = raw_t{};
+      if (kept[k]) wr[k][j] = *reinterpret_cast<const raw_t*>(st + (long long)j * p.D);
+    }
   }
+  ConvLane<VEC, W> c;
   c.init(p, d);
-  c.out(win, xv, yv);
-  store_c<VEC>((bf16_t*)p.y + r * p.ldy + d, yv);
-  if (p.state && q.slot >= 0) {
-    c.shift(win, xv);
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) store_c<VEC>(st + (long long)j * p.D, win[j]);
+  for (int k = 0; k < SEQS; ++k) {
+    if (!live[k]) continue;
+    float win[W - 1][VEC], xv[VEC], yv[VEC];
+    load_c<VEC>((const bf16_t*)&xr[k], xv);
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) load_c<VEC>((const bf16_t*)&wr[k][j], win[j]);
+    c.out(win, xv, yv);
+    store_c<VEC>((bf16_t*)p.y + (long long)(r0 + k) * p.ldy + d, yv);
+    if (p.state && slot[k] >= 0) {                 // the kept inputs move up by one, as they are
+      bf16_t* st = (bf16_t*)p.state + slot[k] * p.ld_slot + d;
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j) *reinterpret_cast<raw_t*>(st + (long long)j * p.D) = j + 1 < W - 1 ? wr[k][j + 1 < W - 1 ? j + 1 : 0] : xr[k];
+    }
   }
 }
 
 template <int VEC, int W>
 void launch_conv(const ActhCausalConvDesc& d, hipStream_t stream) {
   if (!d.starts && d.nseq == d.T) {
-    const long long n = (long long)d.T * ((d.D + VEC - 1) / VEC);
-    causal_conv_step_kernel<VEC, W><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(d);
+    const unsigned bx = (unsigned)((d.D + 256 * VEC - 1) / (256 * VEC));
+    if ((long long)bx * d.T >= 1024) causal_conv_step_kernel<VEC, W, CSTEP><<<dim3(bx, (unsigned)((d.T + CSTEP - 1) / CSTEP)), 256, 0, stream>>>(d);
+    else causal_conv_step_kernel<VEC, W, 1><<<dim3(bx, (unsigned)d.T), 256, 0, stream>>>(d);
   } else {
     const dim3 grid((unsigned)((d.T + CT - 1) / CT), (unsigned)((d.D + 64 * VEC - 1) / (64 * VEC)));
     causal_conv_kernel<VEC, W><<<grid, 64, 0, stream>>>(d);
@@ -274,18 +293,92 @@ __device__ __forceinline__ float load_any(const void* p, long long i, int f32) {
   return f32 ? ((const float*)p)[i] : bf2f(((const bf16_t*)p)[i]);
 }
 
-// A long axis with few rows is cut into chunks of rows:
-//   pass 1 (LOCAL)   every chunk from a zero state (or from the sequence that starts in it): its end state and the sum
-//                    of its time steps, which gives the chunk's decay exp(A sum dt) for all states at once;
-//   carry            the states at the chunks' starts, one after the other, a lane per channel and state;
-//   pass 2 (FINAL)   every chunk from its true start state: outputs and kept states.
-// Chunks are ranges of the row axis and not of a sequence, so their number needs no lengths; a sequence that starts
-// inside a chunk replaces the state there. A chunk that ends where a sequence ends skips pass 1.
+// A long sequence is cut into chunks of at most `len` rows, so that few rows fill the chip as well:
+//   pass 1 (LOCAL)   every chunk but a sequence's last, the first one from the sequence's start state and the others from
+//                    zero: its end state, and the sum of its time steps, which gives its decay exp(A sum dt);
+//   carry            the true states at the chunks' starts, one after the other, a lane per channel and state;
+//   pass 2 (FINAL)   every chunk from its start state: outputs, and the sequence's new state.
+// A sequence of one chunk takes pass 2 alone. Chunk k of sequence i is found on the device from the offsets. The start
+// states of a sequence's chunks lie in consecutive places of the workspace, the first one's among them: pass 2 writes
+// the kept states, so nothing may read them there any more.
 struct Chunks {
-  int len, n;                                      // rows a chunk, chunks
-  float* h;                                        // (n, D, N): end states, then start states, then kept states
-  float* s;                                        // (n, D): sums of the time steps
+  int len, n, places;                              // rows a chunk; bounds of the chunks and of the workspace's places
+  float* h;                                        // (places, D, N): end states at the next chunk's place, then start states
+  float* s;                                        // (places, D): sums of the time steps of the chunk before
+  int* kind;                                       // (places): 0 a start state as it is, 1 decays what comes before it
 };
+
+struct Chunk { int i, slot, r0, r1, j, c, place; };     // chunk j of the c of sequence i, rows [r0, r1); i = -1: none
+
+// Lane by lane over the sequences, 64 at a time: prefix sums of their chunks, and of those of sequences of several.
+// idx < 0: the sums over all sequences (r0 chunks, place places).
+template <class P>
+__device__ __forceinline__ Chunk chunk_find(const P& p, const Chunks& ck, int idx) {
+  Chunk k{};
+  k.i = -1;
+  if (!p.starts) {
+    const int L = p.T / p.nseq, c = (L + ck.len - 1) / ck.len;
+    if (idx < 0) {
+      k.r0 = c * p.nseq;
+      k.place = c > 1 ? k.r0 : 0;
+      return k;
+    }
+    if (idx >= c * p.nseq) return k;
+    const int i = idx / c;
+    k.slot = seq_slot(p, i);
+    if (p.slots && k.slot < 0) return k;
+    k.i = i;
+    k.j = idx - i * c;
+    k.c = c;
+    k.place = c > 1 ? i * c : 0;
+    k.r0 = i * L + k.j * ck.len;
+    k.r1 = min(k.r0 + ck.len, i * L + L);
+    return k;
+  }
+  const int lane = threadIdx.x & 63;
+  int before = 0, multi = 0;
+  for (int i0 = 0; i0 < p.nseq; i0 += 64) {
+    const int i = i0 + lane;
+    int s = 0, e = 0, slot = -1, c = 0, len = ck.len;
+    if (i < p.nseq) {
+      s = seq_start(p, i);
+      e = seq_start(p, i + 1);
+      slot = seq_slot(p, i);
+      if (e > s && (!p.slots || slot >= 0)) {      // about equal chunks: a short last one would leave its place idle
+        c = (e - s + ck.len - 1) / ck.len;
+        len = ((e - s + c - 1) / c + 7) & ~7;
+        c = (e - s + len - 1) / len;
+      }
+    }
+    const int m = c > 1 ? c : 0;
+    int x = c, y = m;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int vx = __shfl_up(x, o, 64), vy = __shfl_up(y, o, 64);
+      if (lane >= o) { x += vx; y += vy; }
+    }
+    const int total = __shfl(x, 63, 64);
+    if (idx >= 0 && idx - before < total) {
+      const int at = __ffsll((unsigned long long)__ballot(x > idx - before)) - 1;
+      const int c0 = before + __shfl(x - c, at, 64);
+      k.i = i0 + at;
+      k.c = __shfl(c, at, 64);
+      k.j = idx - c0;
+      k.place = multi + __shfl(y - m, at, 64);
+      k.slot = __shfl(slot, at, 64);
+      len = __shfl(len, at, 64);
+      k.r0 = __shfl(s, at, 64) + k.j * len;
+      k.r1 = min(k.r0 + len, __shfl(e, at, 64));
+      if (k.c > 1 && k.place + k.c > ck.places) k.i = -1;      // offsets that overlap: not more than there is room for
+      return k;
+    }
+    before += total;
+    multi += __shfl(y, 63, 64);
+  }
+  k.r0 = before;
+  k.place = multi;
+  return k;
+}
 
 constexpr int TT = 8;                             // rows of a tile in LDS
 
@@ -309,21 +402,14 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
   __shared__ __align__(16) float2 sx[TT][PITCH];
   __shared__ __align__(16) float sb[TT][NS], sc[LOCAL ? 1 : TT][NS];
   __shared__ __align__(16) float s_bias[CB], s_skip[CB];
-  __shared__ int s_ok[TT];
 
   const int lane = threadIdx.x;
-  const int chunk = blockIdx.x;
-  const int c0 = chunk * ck.len, c1 = min(c0 + ck.len, p.T);
+  const Chunk q = chunk_find(p, ck, blockIdx.x);
+  if (q.i < 0 || (LOCAL && q.j + 1 >= q.c)) return;
+  const int c0 = q.r0, c1 = q.r1;
   const int dg = p.D / p.G, nb = (dg + CB - 1) / CB;
   const int g = blockIdx.y / nb;
   const int d0 = g * dg + (blockIdx.y - g * nb) * CB, d1 = min(d0 + CB, (g + 1) * dg);
-
-  Seq q = seq_find(p, c0);
-  if (LOCAL) {
-    if (c1 >= p.T) return;
-    const Seq last = seq_find(p, c1);              // is the chunk's end state anybody's start state?
-    if (last.i < 0 || last.i >= p.nseq || last.s >= c1 || last.e <= c1) return;
-  }
 
   // ---- loads of a tile, held until the tile before it is done. A lane's places move down TT rows a tile. Rows behind
   // the chunk are not loaded and channels behind the wave's last read that one again: what they leave is never walked
@@ -423,10 +509,12 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
       }
   };
   const long long dn = (long long)p.D * p.N;
-  if (!LOCAL && q.i >= 0 && q.i < p.nseq && q.s < c0 && q.e > c0) load_h(ck.h + chunk * dn);
+  float* const state = p.state + (p.state ? q.slot * p.ld_slot : 0);
+  if (!LOCAL && q.c > 1) load_h(ck.h + (q.place + q.j) * dn);
+  else if (q.j == 0 && p.state && !(p.fresh && p.fresh[q.i])) load_h(state);
   pin();
+  if (LOCAL && q.j == 0) store_h(ck.h + q.place * dn);
 
-  int t = c0;
   __syncthreads();
   for (int b0 = c0; b0 < c1; b0 += TT) {
     const int b1 = min(b0 + TT, c1);
@@ -478,76 +566,45 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
       sb[i / NS][i % NS] = p.bc_f32 ? __uint_as_float(pb[k]) : bf2f((bf16_t)pb[k]);
       if (!LOCAL) sc[i / NS][i % NS] = p.bc_f32 ? __uint_as_float(pc[k]) : bf2f((bf16_t)pc[k]);
     }
-    if (!LOCAL && lane < TT) s_ok[lane] = 0;
     __syncthreads();
     if (b0 + TT < c1) fetch(b0 + TT);
 
-    // ---- walk its rows, sequence by sequence
-    while (t < b1) {
-      if (q.i >= p.nseq) { t = b1; break; }
-      if (q.i < 0 || q.e <= t) {                   // rows that no sequence holds, or an empty sequence
-        if (q.i < 0) t = max(t, min(q.e, b1));
-        if (q.i < 0 && q.e > t) break;
-        q = seq_of(p, q.i + 1);
-        continue;
-      }
-      if (q.s > t) { t = min(q.s, b1); continue; }
-      if (t == q.s) {
-#pragma unroll
-        for (int j = 0; j < CPT; ++j)
-#pragma unroll
-          for (int s = 0; s < SPL; ++s) h[j][s] = 0.0f;
-        if (seq_kept(p, q)) {
-          load_h(p.state + q.slot * p.ld_slot);
-          pin();
-        }
-      }
-      const int e = min(q.e, b1);
-      if (!LOCAL && lane >= t - b0 && lane < e - b0) s_ok[lane] = !p.slots || q.slot >= 0;
+    // ---- walk its rows (reading the next row's values ahead of their use changed nothing, with many waves or with few)
+    const int rows = b1 - b0;
 #pragma unroll 2
-      for (; t < e; ++t) {
-        const int r = t - b0;
-        float B[SPL], y[CPT];
+    for (int r = 0; r < rows; ++r) {
+      float B[SPL], y[CPT];
 #pragma unroll
-        for (int s = 0; s < SPL; s += 4) *reinterpret_cast<float4*>(B + s) = *reinterpret_cast<const float4*>(&sb[r][part * SPL + s]);
-        float C[SPL];
-        if (!LOCAL) {
+      for (int s = 0; s < SPL; s += 4) *reinterpret_cast<float4*>(B + s) = *reinterpret_cast<const float4*>(&sb[r][part * SPL + s]);
+      float C[SPL];
+      if (!LOCAL) {
 #pragma unroll
-          for (int s = 0; s < SPL; s += 4) *reinterpret_cast<float4*>(C + s) = *reinterpret_cast<const float4*>(&sc[r][part * SPL + s]);
+        for (int s = 0; s < SPL; s += 4) *reinterpret_cast<float4*>(C + s) = *reinterpret_cast<const float4*>(&sc[r][part * SPL + s]);
+      }
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) {
+        const float2 x = sx[r][place(j)];
+        if (LOCAL) sum[j] += x.x;
+        float y1 = 0.0f;                           // two chains of sums
+        y[j] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < SPL; ++s) {
+          const float a = __builtin_amdgcn_exp2f(x.x * A[j][s]);
+          h[j][s] = fmaf(a, h[j][s], x.y * B[s]);
+          if (!LOCAL) {
+            if (s & 1) y1 = fmaf(h[j][s], C[s], y1);
+            else y[j] = fmaf(h[j][s], C[s], y[j]);
+          }
         }
+        y[j] += y1;
+      }
+      if (!LOCAL) {
 #pragma unroll
         for (int j = 0; j < CPT; ++j) {
-          const float2 x = sx[r][place(j)];
-          if (LOCAL) sum[j] += x.x;
-          float y1 = 0.0f;
-          y[j] = 0.0f;
 #pragma unroll
-          for (int s = 0; s < SPL; ++s) {
-            const float a = __builtin_amdgcn_exp2f(x.x * A[j][s]);
-            h[j][s] = fmaf(a, h[j][s], x.y * B[s]);
-            if (!LOCAL) {
-              if (s & 1) y1 = fmaf(h[j][s], C[s], y1);
-              else y[j] = fmaf(h[j][s], C[s], y[j]);
-            }
-          }
-          y[j] += y1;
+          for (int o = 1; o < LPC; o <<= 1) y[j] += __shfl_xor(y[j], o, 64);
+          if (part == 0) sx[r][place(j)].x = y[j];
         }
-        if (!LOCAL) {
-#pragma unroll
-          for (int j = 0; j < CPT; ++j) {
-#pragma unroll
-            for (int o = 1; o < LPC; o <<= 1) y[j] += __shfl_xor(y[j], o, 64);
-            if (part == 0) sx[r][place(j)].x = y[j];
-          }
-        }
-      }
-      if (t == q.e) {
-        if (!LOCAL && p.state && q.slot >= 0) {
-          // a sequence that began in another chunk: that chunk may not have read the kept state yet, so the new one
-          // waits in this chunk's own workspace row (its start state has been read) for the last kernel
-          store_h(q.s < c0 ? ck.h + chunk * dn : p.state + q.slot * p.ld_slot);
-        }
-        q = seq_of(p, q.i + 1);
       }
     }
     __syncthreads();
@@ -557,7 +614,7 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
 #pragma unroll
       for (int k = 0; k < E8; ++k) {
         const int piece = lane + 64 * k, r = piece / C8, c = piece % C8, d = d0 + c * 8;
-        if (r >= TT || !s_ok[r < TT ? r : 0] || d >= d1) continue;
+        if (r >= b1 - b0 || d >= d1) continue;
         const long long row = b0 + r;
         float y[8], uf[8], zf[8];
         unpack8(u[k], uf);
@@ -586,178 +643,246 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
     }
   }
   if (LOCAL) {
-    store_h(ck.h + chunk * dn);
+    store_h(ck.h + (q.place + q.j + 1) * dn);
     if (part == 0) {
 #pragma unroll
       for (int j = 0; j < CPT; ++j)
-        if (channel(j) < d1) ck.s[(long long)chunk * p.D + channel(j)] = sum[j];
+        if (channel(j) < d1) ck.s[(long long)(q.place + q.j + 1) * p.D + channel(j)] = sum[j];
     }
+    if (blockIdx.y == 0 && lane == 0) {
+      if (q.j == 0) ck.kind[q.place] = 0;
+      ck.kind[q.place + q.j + 1] = q.j > 0;
+    }
+  } else if (p.state && q.j + 1 == q.c) {
+    store_h(state);
   }
 }
 
-// The states at the chunks' starts: a lane per channel and state walks the chunks. Where a sequence starts inside a
-// chunk nothing passes through it; where a chunk's end state is nobody's start state (pass 1 left it out) zero does.
-__global__ __launch_bounds__(256) void ssm_carry_kernel(const ActhSsmScanDesc p, const Chunks ck) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x, dn = (long long)p.D * p.N;
-  __shared__ int s_kind[256];                       // of 256 chunks: 0 end unused, 1 starts anew inside, 2 passes through
-  const long long ii = i < dn ? i : 0;
-  const int d = (int)(ii / p.N);
-  const float A = p.A[ii] * kLog2e;
-  float h = 0.0f;
-  for (int b = 0; b + 1 < ck.n; b += 256) {
-    __syncthreads();
-    const int c = b + threadIdx.x;
-    if (c + 1 < ck.n) {
-      const int c0 = c * ck.len, c1 = c0 + ck.len;
-      const Seq q = seq_find(p, c1);
-      s_kind[threadIdx.x] = q.i < 0 || q.i >= p.nseq || q.s >= c1 || q.e <= c1 ? 0 : q.s >= c0 ? 1 : 2;
+// The states at the chunks' starts: a lane per channel and state walks the places of all sequences, 16 at a time, the
+// next 16 under way before this ones' stores (loads that were asked for after a store wait for it). 256 places of
+// 640 x 16 states: 8, 16, 32 at a time 44, 40, 37 us, this 33; 74 places of 2560 x 16 states 13.5 us. Bound: the latency
+// of its loads, which few channels leave bare.
+__global__ __launch_bounds__(64) void ssm_carry_kernel(const ActhSsmScanDesc p, const Chunks ck) {
+  const int n = min(chunk_find(p, ck, -1).place, ck.places);
+  const long long i = (long long)blockIdx.x * 64 + threadIdx.x, dn = (long long)p.D * p.N;
+  if (i >= dn || n < 1) return;
+  const int d = (int)(i / p.N);
+  const float A = p.A[i] * kLog2e;
+  constexpr int B = 16;
+  float e[2][B], s[2][B], h = 0.0f;
+  int kind[2][B];
+  auto load = [&](int f, int k) {
+#pragma unroll
+    for (int v = 0; v < B; ++v) {
+      const long long at = min(k + v, n - 1);
+      e[f][v] = ck.h[at * dn + i];
+      s[f][v] = ck.s[at * p.D + d];
+      kind[f][v] = ck.kind[at];
     }
-    __syncthreads();
-    const int n = min(256, ck.n - 1 - b);
-    // loads of 8 chunks at a time, whatever their kind, so that they are all under way together
-    for (int k = 0; k < n; k += 8) {
-      float e[8], s[8];
+  };
+  auto walk = [&](int f, int k) {
 #pragma unroll
-      for (int v = 0; v < 8; ++v) {
-        const long long at = b + min(k + v, n - 1);
-        e[v] = ck.h[at * dn + ii];
-        s[v] = ck.s[at * p.D + d];
-      }
-#pragma unroll
-      for (int v = 0; v < 8; ++v) {
-        if (k + v >= n) break;
-        const int kind = s_kind[k + v];
-        if (i < dn) ck.h[(b + k + v) * dn + ii] = h;
-        const float keep = kind == 2 ? __builtin_amdgcn_exp2f(A * s[v]) * h : 0.0f;
-        h = kind ? keep + e[v] : 0.0f;
-      }
+    for (int v = 0; v < B; ++v) {
+      if (k + v >= n) break;
+      h = kind[f][v] ? fmaf(__builtin_amdgcn_exp2f(A * s[f][v]), h, e[f][v]) : e[f][v];
+      if (kind[f][v]) ck.h[(long long)(k + v) * dn + i] = h;
     }
-  }
-  if (i < dn) ck.h[(long long)(ck.n - 1) * dn + ii] = h;
-}
-
-// the kept states of the sequences that span chunks, from the workspace row of the chunk they end in
-__global__ __launch_bounds__(256) void ssm_keep_kernel(const ActhSsmScanDesc p, const Chunks ck) {
-  const int c = blockIdx.y, c0 = c * ck.len, c1 = min(c0 + ck.len, p.T);
-  const Seq q = seq_find(p, c0);
-  if (q.i < 0 || q.i >= p.nseq || q.s >= c0 || q.e <= c0 || q.e > c1 || q.slot < 0) return;
-  const long long dn = (long long)p.D * p.N;
-#pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    const long long i = ((long long)blockIdx.x * 16 + k) * 256 + threadIdx.x;
-    if (i < dn) p.state[q.slot * p.ld_slot + i] = ck.h[c * dn + i];
+  };
+  load(0, 0);
+  for (int k = 0; k < n; k += 2 * B) {
+    load(1, k + B);
+    walk(0, k);
+    load(0, k + 2 * B);
+    walk(1, k + B);
   }
 }
 
-// One row a sequence: a lane holds VN states of one channel (VN = 4: a 16-byte load), LPC lanes a channel, and takes
-// SEQS sequences so that A is read once for them. Bound: the states' bytes, in and out; few rows: the launch.
-template <int VN, int LPC>
-__global__ __launch_bounds__(256) void ssm_step_kernel(const ActhSsmScanDesc p, int seqs) {
+constexpr int STEPS = 2;                           // 512 sequences x 5120 channels x 16 states: 1, 2, 4, 8: 87, 72, 75, 93 us
+
+// One row a sequence: a lane holds VN states of one channel (VN = 4: a 16-byte load), LPC lanes a channel, and takes SEQS
+// sequences, all of whose loads are under way before the first is used, so that A is read once for them. VBC: four
+// values of B (and of C) in one load. Bound: the states' bytes, in and out; few rows: the launch.
+template <int VN, int LPC, int SEQS, bool VBC>
+__global__ __launch_bounds__(256) void ssm_step_kernel(const ActhSsmScanDesc p) {
   const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
   const int d = (int)(at / LPC), part = (int)(at % LPC);
   const bool in = d < p.D;
   const int dd = in ? d : 0, n0 = part * VN, g = dd / (p.D / p.G);
   const bool on = in && n0 < p.N;                  // N % VN == 0
-  float A[VN];
+  const int nn = on ? n0 : 0;                      // lanes without a state of their own read the first ones
+  const int r0 = blockIdx.y * SEQS;
+
+  int slot[SEQS];
+  bool kept[SEQS], live[SEQS];
+  float h[SEQS][VN];
+  uint32_t dr[SEQS], br[SEQS][VN], cr[SEQS][VN];   // raw: a conversion here would wait for its load
+  bf16_t ur[SEQS], zr[SEQS];
 #pragma unroll
-  for (int v = 0; v < VN; ++v) A[v] = on ? p.A[(long long)dd * p.N + n0 + v] * kLog2e : 0.0f;
-  const float bias = p.delta_bias ? p.delta_bias[dd] : 0.0f, skip = p.Dskip ? p.Dskip[dd] : 0.0f;
-  const int r1 = (int)min((long long)p.T, ((long long)blockIdx.y + 1) * seqs);
-  for (int r = blockIdx.y * seqs; r < r1; ++r) {
+  for (int k = 0; k < SEQS; ++k) {
+    const int r = min(r0 + k, p.T - 1);
     const Seq q = seq_of(p, r);
-    if (p.slots && q.slot < 0) continue;
+    live[k] = r0 + k < p.T && (!p.slots || q.slot >= 0);
+    slot[k] = q.slot;
+    kept[k] = seq_kept(p, q);
     const long long row = r;
-    float dt = load_any(p.delta, row * p.ld_delta + dd, p.delta_f32) + bias;
-    const float u = bf2f(((const bf16_t*)p.u)[row * p.ldu + dd]);
-    float h[VN], B[VN], C[VN];
+    const float* st = p.state + (q.slot < 0 ? 0 : q.slot) * p.ld_slot + (long long)dd * p.N + nn;
 #pragma unroll
-    for (int v = 0; v < VN; ++v) { h[v] = 0.0f; B[v] = 0.0f; C[v] = 0.0f; }
-    float* st = p.state + (q.slot < 0 ? 0 : q.slot) * p.ld_slot + (long long)dd * p.N + n0;
-    if (on) {
-      if (seq_kept(p, q)) {
-        if constexpr (VN == 4) *reinterpret_cast<float4*>(h) = *reinterpret_cast<const float4*>(st);
-        else h[0] = st[0];
+    for (int v = 0; v < VN; ++v) h[k][v] = 0.0f;
+    if (kept[k]) {
+      if constexpr (VN == 4) *reinterpret_cast<float4*>(h[k]) = *reinterpret_cast<const float4*>(st);
+      else h[k][0] = st[0];
+    }
+    ur[k] = ((const bf16_t*)p.u)[row * p.ldu + dd];
+    zr[k] = 0;
+    if (p.z) zr[k] = ((const bf16_t*)p.z)[row * p.ldz + dd];
+    if (p.delta_f32) dr[k] = ((const uint32_t*)p.delta)[row * p.ld_delta + dd];
+    else dr[k] = ((const bf16_t*)p.delta)[row * p.ld_delta + dd];
+    const long long ob = row * p.ldb + g * p.N + nn, oc = row * p.ldc + g * p.N + nn;
+    if constexpr (VBC) {
+      if (p.bc_f32) {
+        *reinterpret_cast<uint4*>(br[k]) = *reinterpret_cast<const uint4*>((const uint32_t*)p.B + ob);
+        *reinterpret_cast<uint4*>(cr[k]) = *reinterpret_cast<const uint4*>((const uint32_t*)p.C + oc);
+      } else {
+        *reinterpret_cast<uint2*>(br[k]) = *reinterpret_cast<const uint2*>((const bf16_t*)p.B + ob);
+        *reinterpret_cast<uint2*>(cr[k]) = *reinterpret_cast<const uint2*>((const bf16_t*)p.C + oc);
       }
+    } else {
 #pragma unroll
       for (int v = 0; v < VN; ++v) {
-        B[v] = load_any(p.B, row * p.ldb + g * p.N + n0 + v, p.bc_f32);
-        C[v] = load_any(p.C, row * p.ldc + g * p.N + n0 + v, p.bc_f32);
+        if (p.bc_f32) {
+          br[k][v] = ((const uint32_t*)p.B)[ob + v];
+          cr[k][v] = ((const uint32_t*)p.C)[oc + v];
+        } else {
+          br[k][v] = ((const bf16_t*)p.B)[ob + v];
+          cr[k][v] = ((const bf16_t*)p.C)[oc + v];
+        }
       }
     }
+  }
+  float A[VN];
+#pragma unroll
+  for (int v = 0; v < VN; ++v) A[v] = p.A[(long long)dd * p.N + nn + v] * kLog2e;
+  const float bias = p.delta_bias ? p.delta_bias[dd] : 0.0f, skip = p.Dskip ? p.Dskip[dd] : 0.0f;
+
+#pragma unroll
+  for (int k = 0; k < SEQS; ++k) {
+    if (!live[k]) continue;
+    float B[VN], C[VN];
+#pragma unroll
+    for (int v = 0; v < VN; ++v) {
+      if (p.bc_f32) {
+        B[v] = __uint_as_float(br[k][v]);
+        C[v] = __uint_as_float(cr[k][v]);
+      } else if constexpr (VBC) {
+        B[v] = v & 1 ? hi16f(br[k][v >> 1]) : lo16f(br[k][v >> 1]);
+        C[v] = v & 1 ? hi16f(cr[k][v >> 1]) : lo16f(cr[k][v >> 1]);
+      } else {
+        B[v] = bf2f((bf16_t)br[k][v]);
+        C[v] = bf2f((bf16_t)cr[k][v]);
+      }
+    }
+    float dt = (p.delta_f32 ? __uint_as_float(dr[k]) : bf2f((bf16_t)dr[k])) + bias;
+    const float u = bf2f(ur[k]);
     if (p.softplus) dt = softplus16(dt);
     const float du = dt * u;
     float y = 0.0f;
 #pragma unroll
     for (int v = 0; v < VN; ++v) {
-      h[v] = fmaf(__builtin_amdgcn_exp2f(dt * A[v]), h[v], du * B[v]);
-      y = fmaf(h[v], C[v], y);
+      h[k][v] = fmaf(__builtin_amdgcn_exp2f(dt * A[v]), h[k][v], du * B[v]);
+      y = fmaf(h[k][v], C[v], y);
     }
+    if (!on) y = 0.0f;
 #pragma unroll
     for (int o = 1; o < LPC; o <<= 1) y += __shfl_xor(y, o, 64);
-    if (on && p.state && q.slot >= 0) {
-      if constexpr (VN == 4) *reinterpret_cast<float4*>(st) = make_float4(h[0], h[1], h[2], h[3]);
-      else st[0] = h[0];
+    if (on && p.state && slot[k] >= 0) {
+      float* st = p.state + slot[k] * p.ld_slot + (long long)dd * p.N + nn;
+      if constexpr (VN == 4) *reinterpret_cast<float4*>(st) = make_float4(h[k][0], h[k][1], h[k][2], h[k][3]);
+      else st[0] = h[k][0];
     }
     if (in && part == 0) {
       y = fmaf(skip, u, y);
-      if (p.z) y *= silu16(bf2f(((const bf16_t*)p.z)[row * p.ldz + dd]));
-      ((bf16_t*)p.y)[row * p.ldy + dd] = f2bf(y);
+      if (p.z) y *= silu16(bf2f(zr[k]));
+      ((bf16_t*)p.y)[(long long)(r0 + k) * p.ldy + dd] = f2bf(y);
     }
   }
 }
 
-template <int VN, int LPC>
-void launch_step(const ActhSsmScanDesc& d, hipStream_t stream) {
-  const int seqs = d.T >= 256 ? 4 : 1;
-  const dim3 grid((unsigned)(((long long)d.D * LPC + 255) / 256), (unsigned)((d.T + seqs - 1) / seqs));
-  ssm_step_kernel<VN, LPC><<<grid, 256, 0, stream>>>(d, seqs);
+template <int VN, int LPC, int SEQS, bool VBC>
+void launch_step2(const ActhSsmScanDesc& d, hipStream_t stream) {
+  const dim3 grid((unsigned)(((long long)d.D * LPC + 255) / 256), (unsigned)((d.T + SEQS - 1) / SEQS));
+  ssm_step_kernel<VN, LPC, SEQS, VBC><<<grid, 256, 0, stream>>>(d);
 }
 
-// channels a wave takes, by the number of states
-int scan_cb(int N) { return N <= 16 ? 64 : N <= 32 ? 32 : 16; }
+// several sequences a lane once there are enough lanes to fill the chip without it
+template <int VN, int LPC>
+void launch_step(const ActhSsmScanDesc& d, bool vbc, hipStream_t stream) {
+  const bool many = (long long)d.D * LPC / 64 * (d.T / STEPS) >= 4096;
+  if constexpr (VN == 4) {
+    if (vbc) many ? launch_step2<VN, LPC, STEPS, true>(d, stream) : launch_step2<VN, LPC, 1, true>(d, stream);
+    else many ? launch_step2<VN, LPC, STEPS, false>(d, stream) : launch_step2<VN, LPC, 1, false>(d, stream);
+  } else {
+    many ? launch_step2<VN, LPC, STEPS, false>(d, stream) : launch_step2<VN, LPC, 1, false>(d, stream);
+  }
+}
 
+// Few rows and channels: two lanes a channel. 300 x 640: 51 against 45 us, 2000 x 1280: 74 against 70, 16384 x 640: 133
+// against 148.
+bool scan_small(int N, int T, int D) { return N > 8 && N <= 16 && (long long)T / 64 * ((D + 63) / 64) < 2048; }
+
+// channels a wave takes
+int scan_cb(int N, int T, int D) { return N <= 16 ? (scan_small(N, T, D) ? 32 : 64) : N <= 32 ? 32 : 16; }
+
+// Chunks that give one round of the three waves that fit each of the 1024 SIMDs. Ragged ones, which differ in length, are
+// made half as long (16384 x 5120 in 19 sequences: 775 -> 675 us), but not under 112 rows, where pass 1 leaves out too
+// little (8192 x 2560 in 8: 173 us, of 64 rows 194). Few rows: chunks of 16, each wave being mostly latency (300 x 640 of
+// 64, 32, 16 rows: 45, 31, 25 us).
+constexpr int MINLEN = 16;
 Chunks plan(int T, int D, int N, int G, int nseq, int ragged) {
   Chunks c{};
-  const int cb = scan_cb(N);
+  const int cb = scan_cb(N, T, D);
   const long long waves = (long long)G * ((D / G + cb - 1) / cb);
-  const int L = T / nseq;
-  if (!ragged && (nseq == 1 ? T <= 128 : waves * nseq >= 1024 || L <= 64)) {
+  const int L = ragged ? T : T / nseq;             // the longest sequence there can be
+  long long n = 3072 / waves;                      // chunks of all rows
+  if (!ragged) n /= nseq;                          // of one sequence
+  if (n < 1) n = 1;
+  long long len = (L + n - 1) / n;
+  if (ragged && len > 112) len = len / 2 > 112 ? len / 2 : 112;
+  len = (len + TT - 1) / TT * TT;
+  if (len < MINLEN) len = MINLEN;
+  if (L <= 2 * MINLEN || len >= L) {
     c.len = L;
     c.n = nseq;
     return c;
   }
-  long long n = 3072 / waves;                      // one round of the three waves that fit each of 1024 SIMDs
-  if (n < 1) n = 1;
-  long long len = (T + n - 1) / n;
-  len = (len + 15) / 16 * 16;
-  if (len < 64) len = 64;
-  while (T / len >= 65535) len *= 2;               // the chunks are one launch's second dimension
   c.len = (int)len;
-  c.n = (int)((T + len - 1) / len);
+  if (ragged) {
+    c.n = (int)(T / len + nseq);
+    c.places = (int)(2 * (T / len));               // a sequence of several chunks is longer than one
+  } else {
+    c.n = c.places = (int)((L + len - 1) / len * nseq);
+  }
   return c;
 }
 
 template <int SPL, int LPC, int CPT, bool VEC>
-void launch_scan(const ActhSsmScanDesc& d, const Chunks& ck, bool chunked, hipStream_t stream) {
+void launch_scan(const ActhSsmScanDesc& d, const Chunks& ck, hipStream_t stream) {
   constexpr int CB = 64 / LPC * CPT;
   const dim3 grid((unsigned)ck.n, (unsigned)(d.G * ((d.D / d.G + CB - 1) / CB)));
-  if (chunked) {
+  if (ck.places) {
     const long long dn = (long long)d.D * d.N;
     ssm_scan_kernel<SPL, LPC, CPT, true, VEC><<<grid, 64, 0, stream>>>(d, ck);
-    ssm_carry_kernel<<<(unsigned)((dn + 255) / 256), 256, 0, stream>>>(d, ck);
-    ssm_scan_kernel<SPL, LPC, CPT, false, VEC><<<grid, 64, 0, stream>>>(d, ck);
-    if (d.state) ssm_keep_kernel<<<dim3((unsigned)((dn + 4095) / 4096), (unsigned)ck.n), 256, 0, stream>>>(d, ck);
-  } else {
-    ssm_scan_kernel<SPL, LPC, CPT, false, VEC><<<grid, 64, 0, stream>>>(d, ck);
+    ssm_carry_kernel<<<(unsigned)((dn + 63) / 64), 64, 0, stream>>>(d, ck);
   }
+  ssm_scan_kernel<SPL, LPC, CPT, false, VEC><<<grid, 64, 0, stream>>>(d, ck);
 }
 
 template <bool VEC>
-void launch_scan_n(const ActhSsmScanDesc& d, const Chunks& ck, bool chunked, hipStream_t stream) {
-  if (d.N <= 8) launch_scan<8, 1, 1, VEC>(d, ck, chunked, stream);
-  else if (d.N <= 16) launch_scan<16, 1, 1, VEC>(d, ck, chunked, stream);
-  else if (d.N <= 32) launch_scan<16, 2, 1, VEC>(d, ck, chunked, stream);
-  else launch_scan<16, 4, 1, VEC>(d, ck, chunked, stream);
+void launch_scan_n(const ActhSsmScanDesc& d, const Chunks& ck, hipStream_t stream) {
+  if (d.N <= 8) launch_scan<8, 1, 1, VEC>(d, ck, stream);
+  else if (scan_small(d.N, d.T, d.D)) launch_scan<8, 2, 1, VEC>(d, ck, stream);
+  else if (d.N <= 16) launch_scan<16, 1, 1, VEC>(d, ck, stream);
+  else if (d.N <= 32) launch_scan<16, 2, 1, VEC>(d, ck, stream);
+  else launch_scan<16, 4, 1, VEC>(d, ck, stream);
 }
 
 bool al16(const void* p, long long ld_bytes) { return !p || (((uintptr_t)p | (uintptr_t)ld_bytes) % 16) == 0; }
@@ -775,13 +900,14 @@ bool seqs_ok(int T, int nseq, const int* starts, const int* slots, const void* s
 extern "C" int acth_causal_conv(const ActhCausalConvDesc* d, hipStream_t stream) {
   if (!d || d->T < 0) return ACTH_EINVAL;
   if (d->T == 0) return ACTH_OK;
+  if (d->T > (1 << 28) || d->nseq > (1 << 28)) return ACTH_EINVAL;
   if (!d->x || !d->w || !d->y || d->D < 1 || d->W < 2 || d->W > 4) return ACTH_EINVAL;
   if (!seqs_ok(d->T, d->nseq, d->starts, d->slots, d->state, d->nslots)) return ACTH_EINVAL;
   if ((d->T > 1 && (d->ldx < d->D || d->ldy < d->D)) || (d->state && d->ld_slot < (long long)(d->W - 1) * d->D))
     return ACTH_EINVAL;
-  if (d->D > (1 << 25) || (d->T + CT - 1) / CT > (1 << 30)) return ACTH_EINVAL;
+  if (d->D > (1 << 25)) return ACTH_EINVAL;
   const bool vec = d->D % 8 == 0 && al16(d->x, d->ldx * 2) && al16(d->y, d->ldy * 2) && al16(d->state, d->ld_slot * 2);
-  if (!vec && d->D > 65535 * 64) return ACTH_EINVAL;
+  if ((!vec && d->D > 65535 * 64) || (!d->starts && d->nseq == d->T && d->T > 65535)) return ACTH_EINVAL;
   if (vec) {
     if (d->W == 2) launch_conv<8, 2>(*d, stream);
     else if (d->W == 3) launch_conv<8, 3>(*d, stream);
@@ -798,13 +924,13 @@ extern "C" int acth_causal_conv(const ActhCausalConvDesc* d, hipStream_t stream)
 extern "C" size_t acth_ssm_scan_workspace_size(int T, int D, int N, int G, int nseq, int ragged) {
   if (T < 1 || D < 1 || N < 1 || N > 64 || G < 1 || D % G || nseq < 1 || (!ragged && T % nseq)) return 0;
   const Chunks c = plan(T, D, N, G, nseq, ragged);
-  if (c.n < 2 || (!ragged && c.n == nseq && c.len == T / nseq)) return 0;
-  return (size_t)c.n * ((size_t)D * N + D) * 4;
+  return (size_t)c.places * ((size_t)D * N + D + 1) * 4;
 }
 
 extern "C" int acth_ssm_scan(const ActhSsmScanDesc* d, hipStream_t stream) {
   if (!d || d->T < 0) return ACTH_EINVAL;
   if (d->T == 0) return ACTH_OK;
+  if (d->T > (1 << 28) || d->nseq > (1 << 28)) return ACTH_EINVAL;
   if (!d->u || !d->delta || !d->A || !d->B || !d->C || !d->y) return ACTH_EINVAL;
   if (d->D < 1 || d->N < 1 || d->N > 64 || d->G < 1 || d->D % d->G) return ACTH_EINVAL;
   if (!seqs_ok(d->T, d->nseq, d->starts, d->slots, d->state, d->nslots)) return ACTH_EINVAL;
@@ -813,17 +939,19 @@ extern "C" int acth_ssm_scan(const ActhSsmScanDesc* d, hipStream_t stream) {
                    d->ldc < gn)) return ACTH_EINVAL;
   if (d->state && d->ld_slot < (long long)d->D * d->N) return ACTH_EINVAL;
   if (!d->starts && d->nseq == d->T) {
-    if (d->T > 65535 * 4) return ACTH_EINVAL;
+    if (d->T > 65535) return ACTH_EINVAL;
+    const int bsz = d->bc_f32 ? 4 : 2;             // four values of B and of C in one load
+    const bool vbc = (((uintptr_t)d->B | (uintptr_t)d->C | (uintptr_t)(d->ldb * bsz) | (uintptr_t)(d->ldc * bsz)) % (4 * bsz)) == 0;
     if (d->N % 4 == 0 && al16(d->state, d->ld_slot * 4)) {
-      if (d->N <= 8) launch_step<4, 2>(*d, stream);
-      else if (d->N <= 16) launch_step<4, 4>(*d, stream);
-      else if (d->N <= 32) launch_step<4, 8>(*d, stream);
-      else launch_step<4, 16>(*d, stream);
+      if (d->N <= 8) launch_step<4, 2>(*d, vbc, stream);
+      else if (d->N <= 16) launch_step<4, 4>(*d, vbc, stream);
+      else if (d->N <= 32) launch_step<4, 8>(*d, vbc, stream);
+      else launch_step<4, 16>(*d, vbc, stream);
     } else {
-      if (d->N <= 8) launch_step<1, 8>(*d, stream);
-      else if (d->N <= 16) launch_step<1, 16>(*d, stream);
-      else if (d->N <= 32) launch_step<1, 32>(*d, stream);
-      else launch_step<1, 64>(*d, stream);
+      if (d->N <= 8) launch_step<1, 8>(*d, false, stream);
+      else if (d->N <= 16) launch_step<1, 16>(*d, false, stream);
+      else if (d->N <= 32) launch_step<1, 32>(*d, false, stream);
+      else launch_step<1, 64>(*d, false, stream);
     }
     ACTH_CHECK_LAUNCH();
     return ACTH_OK;
@@ -833,13 +961,14 @@ extern "C" int acth_ssm_scan(const ActhSsmScanDesc* d, hipStream_t stream) {
   if (need) {
     if (!d->ws || d->ws_bytes < (long long)need) return ACTH_EINVAL;
     ck.h = d->ws;
-    ck.s = d->ws + (size_t)ck.n * d->D * d->N;
+    ck.s = ck.h + (size_t)ck.places * d->D * d->N;
+    ck.kind = (int*)(ck.s + (size_t)ck.places * d->D);
   }
   if (d->G * ((d->D / d->G + 15) / 16) > 65535) return ACTH_EINVAL;
   const bool vec = d->D / d->G % 8 == 0 && al16(d->u, d->ldu * 2) && al16(d->delta, d->ld_delta * (d->delta_f32 ? 4 : 2)) &&
                   al16(d->z, d->ldz * 2) && al16(d->y, d->ldy * 2);
-  if (vec) launch_scan_n<true>(*d, ck, need != 0, stream);
-  else launch_scan_n<false>(*d, ck, need != 0, stream);
+  if (vec) launch_scan_n<true>(*d, ck, stream);
+  else launch_scan_n<false>(*d, ck, stream);
   ACTH_CHECK_LAUNCH();
   return ACTH_OK;
 }

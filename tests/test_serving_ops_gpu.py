@@ -580,3 +580,20 @@ def test_refusals(dev):
             pytest.fail(f"call {k} was not refused")
     for y in (x, g, st, h):
         assert torch.isfinite(y).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 40, 50), (40, 200, 333), (70, 1500, 1001), (700, 1030, 517)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_gemm_fp8_rows_at_any_address(dev, M, N, K, f32):
+    """Operands inside wider rows, at odd offsets and pitches, with values beside them that must not enter."""
+    big = torch.full((M, K + 11), 448.0).to(ops.FP8)
+    wide = torch.full((N, K + 7), 448.0).to(ops.FP8)
+    big[:, 5:5 + K] = torch.randn(M, K).to(ops.FP8)
+    wide[:, 3:3 + K] = torch.randn(N, K).to(ops.FP8)
+    s, ws = 0.5 + torch.rand(M, -(-K // 128)), 0.5 + torch.rand(-(-N // 128), -(-K // 128))
+    a, w = big.to(dev)[:, 5:5 + K], wide.to(dev)[:, 3:3 + K]
+    out = ops.gemm_fp8(a, s.to(dev), w, ws.to(dev), out_f32=f32)
+    A, W = wide_of(big[:, 5:5 + K], s, 1), wide_of(wide[:, 3:3 + K], ws, 128)
+    want = A @ W.t()
+    tol = (A.abs() @ W.abs().t()) * (K + 8) * U
+    near(out, want, tol if f32 else tol + want.abs() * half() + least_normal() + unit_loss(A, W, dev))
