@@ -194,3 +194,26 @@ __device__ __forceinline__ float wave_max(float v) {
   for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
   return v;
 }
+
+// 16 bytes at any 2-byte (16-bit data) or 4-byte (fp32) address, in one access
+struct __attribute__((packed, aligned(2))) Any16 { uint32_t v[4]; };
+
+__device__ __forceinline__ uint4 load16_at(const void* p) {
+  const Any16 a = *reinterpret_cast<const Any16*>(p);
+  return make_uint4(a.v[0], a.v[1], a.v[2], a.v[3]);
+}
+
+__device__ __forceinline__ void store16_at(void* p, const uint4 v) {
+  Any16 a;
+  a.v[0] = v.x; a.v[1] = v.y; a.v[2] = v.z; a.v[3] = v.w;
+  *reinterpret_cast<Any16*>(p) = a;
+}
+
+// v moved down by n 16-bit places (0 .. 7), zeros above
+__device__ __forceinline__ uint4 down16(const uint4 v, int n) {
+  if (n == 0) return v;
+  const unsigned long long lo = v.x | (unsigned long long)v.y << 32, hi = v.z | (unsigned long long)v.w << 32;
+  const int s = 16 * n;
+  const unsigned long long l = s < 64 ? (lo >> s) | (hi << (64 - s)) : hi >> (s - 64), h = s < 64 ? hi >> s : 0;
+  return make_uint4((uint32_t)l, (uint32_t)(l >> 32), (uint32_t)h, (uint32_t)(h >> 32));
+}

@@ -6,7 +6,8 @@
 // One pass over the data: a row stays in its lanes' registers between the sum of squares and the output, so each
 // input is read once and each output written once. A lane holds chunks of 8 columns (one 16-byte load of 16-bit
 // data), 16 neighbouring lanes hold one block of 128, so a block's maximum is four lane exchanges and needs no LDS.
-// Bound: HBM bandwidth; a few rows: the launch.
+// Bound: HBM bandwidth (32768 x 5120, residual in 16 bits, 8-bit output: 216 us, 5.5 TB/s; 9216 x 1280, fp32 residual: 28 us,
+// 5.0 TB/s; a large copy on this card: 4.8 TB/s read and written); a few rows: the launch (1 x 2560: 3.3 us).
 #include "common.h"
 
 namespace {
@@ -40,14 +41,74 @@ __device__ __forceinline__ uint2 to_eight8(const float* y, float inv) {
   return make_uint2((uint32_t)lo, (uint32_t)hi);
 }
 
+// 8 columns of which n are the row's: 16-bit and fp32
+template <bool WHOLE>
+__device__ __forceinline__ uint4 load8(const bf16_t* p, int n) {
+  if (WHOLE) return *reinterpret_cast<const uint4*>(p);
+  if (n >= 8) return load16_at(p);
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 7; ++e)
+    if (e < n) w[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <bool WHOLE>
+__device__ __forceinline__ void load8f(const float* p, int n, float4& a, float4& b) {
+  if (WHOLE) {
+    a = *reinterpret_cast<const float4*>(p);
+    b = *reinterpret_cast<const float4*>(p + 4);
+  } else if (n >= 8) {
+    const uint4 x = load16_at(p), y = load16_at(p + 4);
+    a = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
+    b = make_float4(__uint_as_float(y.x), __uint_as_float(y.y), __uint_as_float(y.z), __uint_as_float(y.w));
+  } else {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = e < n ? p[e] : 0.0f;
+    a = make_float4(f[0], f[1], f[2], f[3]);
+    b = make_float4(f[4], f[5], f[6], f[7]);
+  }
+}
+
+template <bool WHOLE>
+__device__ __forceinline__ void store8(bf16_t* p, int n, const float* f) {
+  if (WHOLE) {
+    *reinterpret_cast<uint4*>(p) = pack8(f);
+  } else if (n >= 8) {
+    store16_at(p, pack8(f));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (e < n) p[e] = f2bf(f[e]);
+  }
+}
+
+template <bool WHOLE>
+__device__ __forceinline__ void store8f(float* p, int n, const float* f) {
+  if (WHOLE) {
+    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+  } else if (n >= 8) {
+    store16_at(p, make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])));
+    store16_at(p + 4, make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (e < n) p[e] = f[e];
+  }
+}
+
 // TPR lanes share a row (64: one wave, no barrier; 256: one block), CPL chunks of 8 columns each.
-template <int TPR, int CPL, bool EIGHT>
+// WHOLE: every chunk has its 8 columns and lies at a multiple of 16 bytes. Otherwise chunks are loaded from any address
+// and the row's last one, where it is short, column by column.
+template <int TPR, int CPL, bool EIGHT, bool WHOLE>
 __global__ __launch_bounds__(256) void rmsnorm_kernel(const ActhRmsNormDesc p) {
   constexpr int ROWS = 256 / TPR;
   const int lane = threadIdx.x % TPR;
   const long long row = (long long)blockIdx.x * ROWS + threadIdx.x / TPR;
   const bool ok = row < p.M;
-  const int nch = p.C / 8;
+  const int nch = (p.C + 7) / 8;
   const long long r = ok ? row : 0;
   const bf16_t* xr = (const bf16_t*)p.x + r * p.ldx;
 
@@ -57,7 +118,7 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const ActhRmsNormDesc p) {
   for (int c = 0; c < CPL; ++c) {
     const int ch = lane + c * TPR;
     xv[c] = make_uint4(0, 0, 0, 0);
-    if (ch < nch) xv[c] = *reinterpret_cast<const uint4*>(xr + ch * 8);
+    if (ch < nch) xv[c] = load8<WHOLE>(xr + ch * 8, p.C - ch * 8);
   }
   if (p.res && p.res_f32) {
     const float* rr = (const float*)p.res + r * p.ldres;
@@ -65,10 +126,7 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const ActhRmsNormDesc p) {
     for (int c = 0; c < CPL; ++c) {
       const int ch = lane + c * TPR;
       float4 a = make_float4(0, 0, 0, 0), b = a;
-      if (ch < nch) {
-        a = *reinterpret_cast<const float4*>(rr + ch * 8);
-        b = *reinterpret_cast<const float4*>(rr + ch * 8 + 4);
-      }
+      if (ch < nch) load8f<WHOLE>(rr + ch * 8, p.C - ch * 8, a, b);
       unpack8(xv[c], s[c]);
       s[c][0] += a.x; s[c][1] += a.y; s[c][2] += a.z; s[c][3] += a.w;
       s[c][4] += b.x; s[c][5] += b.y; s[c][6] += b.z; s[c][7] += b.w;
@@ -80,7 +138,7 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const ActhRmsNormDesc p) {
     for (int c = 0; c < CPL; ++c) {
       const int ch = lane + c * TPR;
       rv[c] = make_uint4(0, 0, 0, 0);
-      if (ch < nch) rv[c] = *reinterpret_cast<const uint4*>(rr + ch * 8);
+      if (ch < nch) rv[c] = load8<WHOLE>(rr + ch * 8, p.C - ch * 8);
     }
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
@@ -119,40 +177,48 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const ActhRmsNormDesc p) {
     const bool in = ch < nch;
     if (in && p.sum) {
       if (p.res_f32) {
-        float* o = (float*)p.sum + row * p.ldsum + ch * 8;
-        *reinterpret_cast<float4*>(o) = make_float4(s[c][0], s[c][1], s[c][2], s[c][3]);
-        *reinterpret_cast<float4*>(o + 4) = make_float4(s[c][4], s[c][5], s[c][6], s[c][7]);
+        store8f<WHOLE>((float*)p.sum + row * p.ldsum + ch * 8, p.C - ch * 8, s[c]);
       } else {
-        *reinterpret_cast<uint4*>((bf16_t*)p.sum + row * p.ldsum + ch * 8) = pack8(s[c]);
+        store8<WHOLE>((bf16_t*)p.sum + row * p.ldsum + ch * 8, p.C - ch * 8, s[c]);
       }
     }
     float y[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = s[c][e] * rstd;
     if (p.gamma && in) {
-      const float4 a = *reinterpret_cast<const float4*>(p.gamma + ch * 8);
-      const float4 b = *reinterpret_cast<const float4*>(p.gamma + ch * 8 + 4);
+      float4 a, b;
+      load8f<WHOLE>(p.gamma + ch * 8, p.C - ch * 8, a, b);
       y[0] *= a.x; y[1] *= a.y; y[2] *= a.z; y[3] *= a.w;
       y[4] *= b.x; y[5] *= b.y; y[6] *= b.z; y[7] *= b.w;
     }
     if constexpr (EIGHT) {
       uint32_t m = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m = umax_(m, in ? mag(y[e]) : 0u);
+      for (int e = 0; e < 8; ++e) m = umax_(m, in && (WHOLE || ch * 8 + e < p.C) ? mag(y[e]) : 0u);
 #pragma unroll
       for (int o = 1; o < 16; o <<= 1) m = umax_(m, (uint32_t)__shfl_xor((int)m, o, 64));
       if (in) {
         const Block8 b = block_scale(m);
-        *reinterpret_cast<uint2*>((uint8_t*)p.y + row * p.ldy + ch * 8) = to_eight8(y, b.inv);
+        uint8_t* const o = (uint8_t*)p.y + row * p.ldy + ch * 8;
+        const uint2 q = to_eight8(y, b.inv);
+        if (WHOLE || p.C - ch * 8 >= 8) {
+          struct __attribute__((packed, aligned(1))) Any8 { uint32_t v[2]; };
+          if (WHOLE) *reinterpret_cast<uint2*>(o) = q;
+          else *reinterpret_cast<Any8*>(o) = Any8{{q.x, q.y}};
+        } else {
+#pragma unroll
+          for (int e = 0; e < 7; ++e)
+            if (ch * 8 + e < p.C) o[e] = (uint8_t)((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
+        }
         if ((ch & 15) == 0) p.scale[row * p.scale_row + (ch >> 4) * p.scale_blk] = b.scale;
       }
     } else if (in) {
-      *reinterpret_cast<uint4*>((bf16_t*)p.y + row * p.ldy + ch * 8) = pack8(y);
+      store8<WHOLE>((bf16_t*)p.y + row * p.ldy + ch * 8, p.C - ch * 8, y);
     }
   }
 }
 
-// Any width, stride and alignment: a block of 256 walks its row twice, one column a lane (the second read comes from
+// Rows too wide for a block's registers: a block of 256 walks its row twice, one column a lane (the second read comes from
 // L2). A wave takes a block of 128 columns at a time, so a block's maximum stays inside the wave. Columns are summed
 // in a fixed order. A sum or output that lies on an input is written only by the lane that has just read it.
 template <bool EIGHT>
@@ -214,10 +280,12 @@ __global__ __launch_bounds__(256) void rmsnorm_any_kernel(const ActhRmsNormDesc 
 }
 
 template <int TPR, int CPL>
-void launch(const ActhRmsNormDesc& d, hipStream_t stream) {
+void launch(const ActhRmsNormDesc& d, bool whole, hipStream_t stream) {
   const unsigned grid = (unsigned)((d.M + 256 / TPR - 1) / (256 / TPR));
-  if (d.eight) rmsnorm_kernel<TPR, CPL, true><<<grid, 256, 0, stream>>>(d);
-  else rmsnorm_kernel<TPR, CPL, false><<<grid, 256, 0, stream>>>(d);
+  if (d.eight && whole) rmsnorm_kernel<TPR, CPL, true, true><<<grid, 256, 0, stream>>>(d);
+  else if (d.eight) rmsnorm_kernel<TPR, CPL, true, false><<<grid, 256, 0, stream>>>(d);
+  else if (whole) rmsnorm_kernel<TPR, CPL, false, true><<<grid, 256, 0, stream>>>(d);
+  else rmsnorm_kernel<TPR, CPL, false, false><<<grid, 256, 0, stream>>>(d);
 }
 
 bool aligned(const void* p, long long ld_bytes, int to) {
@@ -233,24 +301,22 @@ extern "C" int acth_rmsnorm(const ActhRmsNormDesc* d, hipStream_t stream) {
   if (d->M > 1 && (d->ldx < d->C || d->ldy < d->C || (d->res && d->ldres < d->C) || (d->sum && d->ldsum < d->C)))
     return ACTH_EINVAL;
   const int rs = d->res_f32 ? 4 : 2;
-  const bool vec = d->C % 8 == 0 && aligned(d->x, d->ldx * 2, 16) && aligned(d->res, d->ldres * rs, 16) &&
-                   aligned(d->sum, d->ldsum * rs, 16) && aligned(d->gamma, 0, 16) &&
-                   aligned(d->y, d->ldy * (d->eight ? 1 : 2), d->eight ? 8 : 16);
-  const int nch = d->C / 8;
-  if (!vec || nch > 256 * 8) {
-    if (d->eight) rmsnorm_any_kernel<true><<<d->M, 256, 0, stream>>>(*d);
-    else rmsnorm_any_kernel<false><<<d->M, 256, 0, stream>>>(*d);
-    ACTH_CHECK_LAUNCH();
-    return ACTH_OK;
-  }
-  if (nch <= 64) launch<64, 1>(*d, stream);
-  else if (nch <= 128) launch<64, 2>(*d, stream);
-  else if (nch <= 192) launch<64, 3>(*d, stream);
-  else if (nch <= 256) launch<64, 4>(*d, stream);
-  else if (nch <= 512) launch<256, 2>(*d, stream);
-  else if (nch <= 768) launch<256, 3>(*d, stream);
-  else if (nch <= 1024) launch<256, 4>(*d, stream);
-  else launch<256, 8>(*d, stream);
+  const bool whole = d->C % 8 == 0 && aligned(d->x, d->ldx * 2, 16) && aligned(d->res, d->ldres * rs, 16) &&
+                     aligned(d->sum, d->ldsum * rs, 16) && aligned(d->gamma, 0, 16) &&
+                     aligned(d->y, d->ldy * (d->eight ? 1 : 2), d->eight ? 8 : 16);
+  const int nch = (d->C + 7) / 8;
+  // A wave a row up to 2048 columns, a block above: 32768 x 1280 54 against 69 us, 2048 x 2560 9.1 against 8.6,
+  // 32768 x 5120 225 against 219, 64 x 5120 8.9 against 4.7 (8-bit output, residual in 16 bits).
+  if (nch <= 64) launch<64, 1>(*d, whole, stream);
+  else if (nch <= 128) launch<64, 2>(*d, whole, stream);
+  else if (nch <= 192) launch<64, 3>(*d, whole, stream);
+  else if (nch <= 256) launch<64, 4>(*d, whole, stream);
+  else if (nch <= 512) launch<256, 2>(*d, whole, stream);
+  else if (nch <= 768) launch<256, 3>(*d, whole, stream);
+  else if (nch <= 1024) launch<256, 4>(*d, whole, stream);
+  else if (nch <= 2048) launch<256, 8>(*d, whole, stream);
+  else if (d->eight) rmsnorm_any_kernel<true><<<d->M, 256, 0, stream>>>(*d);
+  else rmsnorm_any_kernel<false><<<d->M, 256, 0, stream>>>(*d);
   ACTH_CHECK_LAUNCH();
   return ACTH_OK;
 }

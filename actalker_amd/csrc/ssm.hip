@@ -71,22 +71,49 @@ __device__ __forceinline__ float silu16(float x) {
 }
 
 // ------------------------------------------------------------------------------------------------ convolution
-// VEC channels a lane (8: one 16-byte load a row; 1: any width and alignment), a wave 64 x VEC channels of 16 rows. The
+// VEC channels a lane (8: one 16-byte load a row, from any address; 1: fewer than 8 channels), a wave 64 x VEC channels of 16 rows. The
 // rows of a tile are loaded before the first is used; the W - 1 rows in front of it are read again (3 of 16, from L2).
 // The tile that holds a sequence's first row also takes the rows that reach back into the kept inputs and writes the
-// new ones, so one lane both reads and writes each kept value. Bound: HBM bandwidth.
+// new ones, so one lane both reads and writes each kept value. Bound: HBM bandwidth (32768 x 5120 x 4 taps, 24 sequences:
+// 154 us, 4.4 TB/s; 8 or 32 rows a tile: 168, 154; channels that fill no 8: 190).
 constexpr int CT = 16;
 
 template <int VEC>
 __device__ __forceinline__ void load_c(const bf16_t* p, float* f) {
-  if constexpr (VEC == 8) unpack8(*reinterpret_cast<const uint4*>(p), f);
+  if constexpr (VEC == 8) unpack8(load16_at(p), f);
   else f[0] = bf2f(*p);
 }
 
+// the channels from `e0` on: the lane of a row's end, where that is short, lies back over its neighbour's channels and
+// leaves those to it
 template <int VEC>
-__device__ __forceinline__ void store_c(bf16_t* p, const float* f) {
-  if constexpr (VEC == 8) *reinterpret_cast<uint4*>(p) = pack8(f);
-  else *p = f2bf(f[0]);
+__device__ __forceinline__ void store_c(bf16_t* p, const float* f, int e0) {
+  if constexpr (VEC == 8) {
+    if (e0 == 0) {
+      store16_at(p, pack8(f));
+    } else {
+#pragma unroll
+      for (int e = 1; e < 8; ++e)
+        if (e >= e0) p[e] = f2bf(f[e]);
+    }
+  } else {
+    *p = f2bf(f[0]);
+  }
+}
+
+template <int VEC> struct Raw { typedef bf16_t type; };
+template <> struct Raw<8> { typedef uint4 type; };
+
+template <int VEC>
+__device__ __forceinline__ typename Raw<VEC>::type load_raw(const bf16_t* p) {
+  if constexpr (VEC == 8) return load16_at(p);
+  else return *p;
+}
+
+template <int VEC>
+__device__ __forceinline__ void from_raw(const typename Raw<VEC>::type v, float* f) {
+  if constexpr (VEC == 8) unpack8(v, f);
+  else f[0] = bf2f(v);
 }
 
 template <int VEC, int W>
@@ -126,8 +153,9 @@ struct ConvLane {
 template <int VEC, int W>
 __global__ __launch_bounds__(64) void causal_conv_kernel(const ActhCausalConvDesc p) {
   const int t0 = blockIdx.x * CT, t1 = min(t0 + CT, p.T);
-  const int d = (blockIdx.y * 64 + threadIdx.x) * VEC;
-  if (d >= p.D) return;
+  const int d_ = (blockIdx.y * 64 + threadIdx.x) * VEC;
+  if (d_ >= p.D) return;
+  const int d = min(d_, p.D - VEC), e0 = d_ - d;
   ConvLane<VEC, W> c;
   c.init(p, d);
   const bf16_t* x = (const bf16_t*)p.x + d;
@@ -144,7 +172,7 @@ __global__ __launch_bounds__(64) void causal_conv_kernel(const ActhCausalConvDes
     for (int k = 0; k < CT; ++k) {
       load_c<VEC>(x + (long long)(t0 + k) * p.ldx, xv);
       c.out(win, xv, yv);
-      store_c<VEC>(y + (long long)(t0 + k) * p.ldy, yv);
+      store_c<VEC>(y + (long long)(t0 + k) * p.ldy, yv, e0);
       c.shift(win, xv);
     }
     return;
@@ -187,7 +215,7 @@ __global__ __launch_bounds__(64) void causal_conv_kernel(const ActhCausalConvDes
       for (int r = a; r < b; ++r) {
         load_c<VEC>(x + (long long)r * p.ldx, xv);
         c.out(win, xv, yv);
-        store_c<VEC>(y + (long long)r * p.ldy, yv);
+        store_c<VEC>(y + (long long)r * p.ldy, yv, e0);
         c.shift(win, xv);
       }
     }
@@ -209,7 +237,7 @@ __global__ __launch_bounds__(64) void causal_conv_kernel(const ActhCausalConvDes
               for (int v = 0; v < VEC; ++v) nv[v] = init[k][v];
             }
         }
-        store_c<VEC>(st + (long long)j * p.D, nv);
+        store_c<VEC>(st + (long long)j * p.D, nv, e0);
       }
     }
     t = max(t, q.e);
@@ -224,10 +252,11 @@ constexpr int CSTEP = 4;                           // 512 sequences x 5120 chann
 // used, so that the weights are read once for them. Bound: the kept inputs' bytes; few rows: the launch.
 template <int VEC, int W, int SEQS>
 __global__ __launch_bounds__(256) void causal_conv_step_kernel(const ActhCausalConvDesc p) {
-  const int d = (blockIdx.x * 256 + threadIdx.x) * VEC;
-  if (d >= p.D) return;
+  const int d_ = (blockIdx.x * 256 + threadIdx.x) * VEC;
+  if (d_ >= p.D) return;
+  const int d = min(d_, p.D - VEC), e0 = d_ - d;
   const int r0 = blockIdx.y * SEQS;
-  typedef typename std::conditional<VEC == 8, uint4, bf16_t>::type raw_t;
+  typedef typename Raw<VEC>::type raw_t;
   raw_t xr[SEQS], wr[SEQS][W - 1];
   int slot[SEQS];
   bool kept[SEQS], live[SEQS];
@@ -238,12 +267,12 @@ __global__ __launch_bounds__(256) void causal_conv_step_kernel(const ActhCausalC
     live[k] = r0 + k < p.T && (!p.slots || q.slot >= 0);
     slot[k] = q.slot;
     kept[k] = seq_kept(p, q);
-    xr[k] = *reinterpret_cast<const raw_t*>((const bf16_t*)p.x + (long long)r * p.ldx + d);
+    xr[k] = load_raw<VEC>((const bf16_t*)p.x + (long long)r * p.ldx + d);
     const bf16_t* st = (const bf16_t*)p.state + (q.slot < 0 ? 0 : q.slot) * p.ld_slot + d;
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) {
       wr[k][j] = raw_t{};
-      if (kept[k]) wr[k][j] = *reinterpret_cast<const raw_t*>(st + (long long)j * p.D);
+      if (kept[k]) wr[k][j] = load_raw<VEC>(st + (long long)j * p.D);
     }
   }
   ConvLane<VEC, W> c;
@@ -252,15 +281,16 @@ __global__ __launch_bounds__(256) void causal_conv_step_kernel(const ActhCausalC
   for (int k = 0; k < SEQS; ++k) {
     if (!live[k]) continue;
     float win[W - 1][VEC], xv[VEC], yv[VEC];
-    load_c<VEC>((const bf16_t*)&xr[k], xv);
+    from_raw<VEC>(xr[k], xv);
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) load_c<VEC>((const bf16_t*)&wr[k][j], win[j]);
+    for (int j = 0; j < W - 1; ++j) from_raw<VEC>(wr[k][j], win[j]);
     c.out(win, xv, yv);
-    store_c<VEC>((bf16_t*)p.y + (long long)(r0 + k) * p.ldy + d, yv);
-    if (p.state && slot[k] >= 0) {                 // the kept inputs move up by one, as they are
+    store_c<VEC>((bf16_t*)p.y + (long long)(r0 + k) * p.ldy + d, yv, e0);
+    if (p.state && slot[k] >= 0) {                 // the kept inputs move up by one
+      c.shift(win, xv);
       bf16_t* st = (bf16_t*)p.state + slot[k] * p.ld_slot + d;
 #pragma unroll
-      for (int j = 0; j < W - 1; ++j) *reinterpret_cast<raw_t*>(st + (long long)j * p.D) = j + 1 < W - 1 ? wr[k][j + 1 < W - 1 ? j + 1 : 0] : xr[k];
+      for (int j = 0; j < W - 1; ++j) store_c<VEC>(st + (long long)j * p.D, win[j], e0);
     }
   }
 }
@@ -382,6 +412,14 @@ __device__ __forceinline__ Chunk chunk_find(const P& p, const Chunks& ck, int id
 
 constexpr int TT = 8;                             // rows of a tile in LDS
 
+// f[i] for i < 8 without addressing registers; 0 behind
+__device__ __forceinline__ float select8(const float* f, int i) {
+  float v = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v = i == e ? f[e] : v;
+  return v;
+}
+
 // A wave takes CB channels of a chunk: SPL states a lane, LPC lanes a channel, CPT channels a lane. A tile's time steps
 // (softplus done once, by the staging lane) and inputs dt u sit in LDS as pairs beside the rows of B and C; the output
 // takes the place of the pair that its own lane has just read. The next tile's rows are loaded while this one is
@@ -389,7 +427,9 @@ constexpr int TT = 8;                             // rows of a tile in LDS
 // Channel c of a row lies at place (c % 8)(CB / 8) + c / 8, and rows are CB bytes further apart than they are long:
 // the staging lanes, which hold 8 neighbouring channels each, then write neighbouring places (laid out by channel they
 // met in 4 banks, 16 at a time), and the walking lanes read one place each.
-// Bound: the vector units, a row, channel and state taking one exponential (8 clocks a wave) and four operations (4 each).
+// Bound: the vector units, a row, channel and state taking one exponential (8 clocks a wave) and four operations (4 each):
+// 8192 x 2560 x 16 states 51 us in pass 2 and 43 in pass 1 if nothing else were done; 101 and 80 measured, the rest being
+// the softplus, gate and conversions of the staging lanes and the waves' waits (the units are 75 - 79 % busy).
 template <int SPL, int LPC, int CPT, bool LOCAL, bool VEC>
 __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p, const Chunks ck) {
   constexpr int CL = 64 / LPC;                     // channels a wave holds at once
@@ -412,12 +452,13 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
   const int d0 = g * dg + (blockIdx.y - g * nb) * CB, d1 = min(d0 + CB, (g + 1) * dg);
 
   // ---- loads of a tile, held until the tile before it is done. A lane's places move down TT rows a tile. Rows behind
-  // the chunk are not loaded and channels behind the wave's last read that one again: what they leave is never walked
-  // or never stored. States behind the last one keep zeros.
+  // the chunk are not loaded; a piece that the group's end cuts is loaded from 8 channels before the end and moved down by
+  // `back`: what lies behind the end is never walked or never stored. States behind the last one keep zeros.
   uint4 pu[E8], pd[E8][2];
   uint32_t pb[NB], pc[NB];                         // raw: a conversion here would wait for its load
   const int dsz = p.delta_f32 ? 4 : 2, bsz = p.bc_f32 ? 4 : 2;
-  const int fr = lane / C8, fd = min(d0 + lane % C8 * 8, d1 - 8);      // (fd: with VEC, d1 - d0 is a multiple of 8)
+  const int fr = lane / C8, fd = min(d0 + lane % C8 * 8, d1 - 8);      // (VEC: a group has 8 channels or more)
+  const int back = min(d0 + lane % C8 * 8 - fd, 7);
   const int gr = lane / NS, gn = lane % NS;
   const bf16_t* at_u = (const bf16_t*)p.u + (long long)(c0 + fr) * p.ldu + fd;
   const char* at_d = (const char*)p.delta + ((long long)(c0 + fr) * p.ld_delta + fd) * dsz;
@@ -432,10 +473,10 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
       for (int k = 0; k < E8; ++k) {
         const int r = fr + 64 / C8 * k;
         if (r < TT && r < left) {
-          pu[k] = *reinterpret_cast<const uint4*>(at_u + (long long)(64 / C8 * k) * p.ldu);
-          const uint4* f = reinterpret_cast<const uint4*>(at_d + (long long)(64 / C8 * k) * p.ld_delta * dsz);
-          pd[k][0] = f[0];
-          if (p.delta_f32) pd[k][1] = f[1];
+          pu[k] = load16_at(at_u + (long long)(64 / C8 * k) * p.ldu);
+          const char* f = at_d + (long long)(64 / C8 * k) * p.ld_delta * dsz;
+          pd[k][0] = load16_at(f);
+          if (p.delta_f32) pd[k][1] = load16_at(f + 16);
         }
       }
       at_u += (long long)TT * p.ldu;
@@ -527,14 +568,18 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
       const bool in = r < TT && b0 + r < b1;
       float uf[8], dl[8];
       if constexpr (VEC) {
-        u[k] = pu[k];
+        u[k] = down16(pu[k], back);
         if (p.delta_f32) {
           dl[0] = __uint_as_float(pd[k][0].x); dl[1] = __uint_as_float(pd[k][0].y);
           dl[2] = __uint_as_float(pd[k][0].z); dl[3] = __uint_as_float(pd[k][0].w);
           dl[4] = __uint_as_float(pd[k][1].x); dl[5] = __uint_as_float(pd[k][1].y);
           dl[6] = __uint_as_float(pd[k][1].z); dl[7] = __uint_as_float(pd[k][1].w);
+          if (back) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dl[e] = select8(dl, e + back);
+          }
         } else {
-          unpack8(pd[k][0], dl);
+          unpack8(down16(pd[k][0], back), dl);
         }
       } else {
         uint32_t w[4] = {0, 0, 0, 0};
@@ -558,7 +603,7 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
         }
       }
       z[k] = make_uint4(0, 0, 0, 0);
-      if (!LOCAL && p.z && VEC && in && d < d1) z[k] = *reinterpret_cast<const uint4*>((const bf16_t*)p.z + row * p.ldz + d);
+      if (!LOCAL && p.z && VEC && in && d < d1) z[k] = load16_at((const bf16_t*)p.z + row * p.ldz + fd);
     }
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
@@ -618,7 +663,7 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
         const long long row = b0 + r;
         float y[8], uf[8], zf[8];
         unpack8(u[k], uf);
-        unpack8(z[k], zf);
+        unpack8(down16(z[k], back), zf);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           y[e] = sx[r][e * C8 + c].x;
@@ -631,8 +676,8 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
             if (d + e < d1) y[e] *= silu16(bf2f(((const bf16_t*)p.z)[row * p.ldz + d + e]));
         }
         bf16_t* o = (bf16_t*)p.y + row * p.ldy + d;
-        if constexpr (VEC) {
-          *reinterpret_cast<uint4*>(o) = pack8(y);
+        if (VEC && back == 0) {
+          store16_at(o, pack8(y));
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -701,7 +746,8 @@ constexpr int STEPS = 2;                           // 512 sequences x 5120 chann
 
 // One row a sequence: a lane holds VN states of one channel (VN = 4: a 16-byte load), LPC lanes a channel, and takes SEQS
 // sequences, all of whose loads are under way before the first is used, so that A is read once for them. VBC: four
-// values of B (and of C) in one load. Bound: the states' bytes, in and out; few rows: the launch.
+// values of B (and of C) in one load. Bound: the states' bytes, in and out (512 x 5120 x 16 states: 72 us,
+// 4.9 TB/s); few rows: the launch (4.2 us).
 template <int VN, int LPC, int SEQS, bool VBC>
 __global__ __launch_bounds__(256) void ssm_step_kernel(const ActhSsmScanDesc p) {
   const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -906,8 +952,8 @@ extern "C" int acth_causal_conv(const ActhCausalConvDesc* d, hipStream_t stream)
   if ((d->T > 1 && (d->ldx < d->D || d->ldy < d->D)) || (d->state && d->ld_slot < (long long)(d->W - 1) * d->D))
     return ACTH_EINVAL;
   if (d->D > (1 << 25)) return ACTH_EINVAL;
-  const bool vec = d->D % 8 == 0 && al16(d->x, d->ldx * 2) && al16(d->y, d->ldy * 2) && al16(d->state, d->ld_slot * 2);
-  if ((!vec && d->D > 65535 * 64) || (!d->starts && d->nseq == d->T && d->T > 65535)) return ACTH_EINVAL;
+  const bool vec = d->D >= 8;
+  if (!d->starts && d->nseq == d->T && d->T > 65535) return ACTH_EINVAL;
   if (vec) {
     if (d->W == 2) launch_conv<8, 2>(*d, stream);
     else if (d->W == 3) launch_conv<8, 3>(*d, stream);
@@ -965,8 +1011,7 @@ extern "C" int acth_ssm_scan(const ActhSsmScanDesc* d, hipStream_t stream) {
     ck.kind = (int*)(ck.s + (size_t)ck.places * d->D);
   }
   if (d->G * ((d->D / d->G + 15) / 16) > 65535) return ACTH_EINVAL;
-  const bool vec = d->D / d->G % 8 == 0 && al16(d->u, d->ldu * 2) && al16(d->delta, d->ld_delta * (d->delta_f32 ? 4 : 2)) &&
-                  al16(d->z, d->ldz * 2) && al16(d->y, d->ldy * 2);
+  const bool vec = d->D / d->G >= 8;
   if (vec) launch_scan_n<true>(*d, ck, stream);
   else launch_scan_n<false>(*d, ck, stream);
   ACTH_CHECK_LAUNCH();

@@ -597,3 +597,25 @@ def test_gemm_fp8_rows_at_any_address(dev, M, N, K, f32):
     want = A @ W.t()
     tol = (A.abs() @ W.abs().t()) * (K + 8) * U
     near(out, want, tol if f32 else tol + want.abs() * half() + least_normal() + unit_loss(A, W, dev))
+
+
+@pytest.mark.parametrize("N,G,z,last,L", [(16, 2, True, True, 75), (16, 1, False, True, 300), (8, 2, False, False, 33), (40, 1, True, True, 1)])
+def test_selective_scan_fn_gate_and_last_state(dev, N, G, z, last, L):
+    """The drop-in's gate, last state and other state counts: (batch, dim, L) operands, fp32 delta, B and C."""
+    from actalker_amd.selective_scan_interface import selective_scan_fn
+    b, dim = 3, 32
+    s = scan_case([L] * b, dim, N, G, "float")
+    y, tol, new, ntol = scan_ref(*(s[k] for k in IN[:6]), s["z"] if z else None, s["delta_bias"], True, cuts_of([L] * b),
+                                 torch.zeros(b, dim, N), [False] * b)
+    seq = lambda t: t.view(b, L, -1).transpose(1, 2).contiguous().to(dev)                            # noqa: E731
+    grp = lambda t: t.reshape(b, L, G, N).permute(0, 2, 3, 1).contiguous().to(dev)                   # noqa: E731
+    out = selective_scan_fn(seq(s["u"]), seq(s["delta"]), s["A"].to(dev), grp(s["B"]), grp(s["C"]), s["D"].to(dev),
+                            z=seq(s["z"]) if z else None, delta_bias=s["delta_bias"].to(dev), delta_softplus=True,
+                            return_last_state=last)
+    if last:
+        out, state = out
+        near(state, new, ntol)
+    assert out.shape == (b, dim, L) and out.dtype == ops.act_dtype()
+    near(out.transpose(1, 2).reshape(b * L, dim), y, tol)
+    with pytest.raises(NotImplementedError):
+        selective_scan_fn(seq(s["u"]), seq(s["delta"]), torch.zeros(dim, 65, device=dev), grp(s["B"]), grp(s["C"]))
