@@ -111,6 +111,12 @@ __device__ __forceinline__ int4 load16_any(const uint8_t* row, int k, int K) {
 // LDS-DMA. 16-byte chunk c of row r lies at chunk c ^ (r % 8) of its 128-byte LDS row, so the 8 lanes of a ds_read_b128
 // group, which read one chunk of 8 rows, meet 8 different bank slots; the DMA, whose LDS side is linear, applies the
 // same exchange to its global side.
+// Bound: 8192^3 takes 531 us (2070 TFLOP/s; the card's library reaches 2690 with one scale for a whole operand, 1260 in 16
+// bits). The matrix unit is busy 47 % of the time and the vector unit, with the scales' multiply-adds, 38 %, at the
+// 1.9 GHz that the card holds under this load; 17 % of the time goes to the LDS-DMA beside the products and 5 % to the
+// multiply-adds (both timed by leaving them out of a copy). Then whole rounds of 256 tiles: 16384 x 2560 is 2.5 of them
+// and costs 3 (253 us, 1700 TFLOP/s). A ring of three 256 x 128 stages, which would be five full rounds there, moves twice
+// the bytes a product through L2 and took 275 us.
 template <int BM, int BN>
 struct Tile {
   static constexpr int WC = BN / 64, WR = 8 / WC;              // waves along n and m
@@ -508,7 +514,7 @@ extern "C" int acth_gemm_fp8(const ActhGemmFp8Desc* d, hipStream_t stream) {
   if (((long long)d->M + 15) / 16 * (((long long)d->N + 31) / 32) > 0x7fffffff && (d->M <= 32 || t128 <= 40)) return ACTH_EINVAL;
   if (t128 > 0x7fffffff) return ACTH_EINVAL;
   // Rounds of the chip: 256 large tiles, or 512 small ones (two blocks a CU), in 1.5 times a small round's time
-  // (42 and 27.5 us at K = 2560). 4096 x 2560: 47 against 50 us, 4096 x 5120: 87 against 72, 16384 x 2560: 253 against 276.
+  // (42 and 27.5 us at K = 2560). 4096 x 2560: 47 against 50 us, 4096 x 5120: 83 against 72, 16384 x 2560 x 5120: 253 against 276.
   const long long r256 = (t256 + 255) / 256, r128 = (t128 + 511) / 512;
   if (d->M <= 32 || t128 <= 40) {                // 256 x 2560 x 2560: 14.6 against 16.2 us, 512 rows: 27.5 against 16.7
     if (dma) d->out_f32 ? launch_few<true, true>(*d, vec_out, stream) : launch_few<false, true>(*d, vec_out, stream);
@@ -518,8 +524,9 @@ extern "C" int acth_gemm_fp8(const ActhGemmFp8Desc* d, hipStream_t stream) {
     else gemm_fp8_any_kernel<false><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
   } else if (d->out_f32) {
     gemm_fp8_kernel<128, 128, true><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
-  } else if (3 * r256 <= 2 * r128) {
-    gemm_fp8_kernel<256, 256, false><<<(unsigned)t256, 512, 0, stream>>>(*d, 8, vec_out);
+  } else if (3 * r256 < 2 * r128) {
+    // row blocks side by side: 4, 8, 16, 32: 450, 480, 480, 513 us at 16384 x 10240 x 2560, 249, 256, 256, 257 at 16384 x 2560 x 5120
+    gemm_fp8_kernel<256, 256, false><<<(unsigned)t256, 512, 0, stream>>>(*d, 4, vec_out);
   } else {
     gemm_fp8_kernel<128, 128, false><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
   }

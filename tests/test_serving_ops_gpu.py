@@ -619,3 +619,16 @@ def test_selective_scan_fn_gate_and_last_state(dev, N, G, z, last, L):
     near(out.transpose(1, 2).reshape(b * L, dim), y, tol)
     with pytest.raises(NotImplementedError):
         selective_scan_fn(seq(s["u"]), seq(s["delta"]), torch.zeros(dim, 65, device=dev), grp(s["B"]), grp(s["C"]))
+
+
+def test_gemm_fp8_more_row_blocks_than_a_group(dev):
+    """Several rounds of large tiles, a last group of fewer row blocks, ragged in every size."""
+    M, N, K = 256 * 33 + 17, 256 * 9 + 40, 144
+    q, s = ops.quant_fp8(low(M, K).to(dev))
+    wq, wsc = ops.pack_fp8(torch.randn(N, K).to(dev) / 12)
+    out = ops.gemm_fp8(q, s, wq, wsc)
+    big = lambda t, c, r: t.float() * c.repeat_interleave(r, 0)[:t.shape[0]].repeat_interleave(128, 1)[:, :K]     # noqa: E731
+    A, W = big(q, s, 1), big(wq, wsc, 128)
+    want, size = (A @ W.t()).cpu().double(), (A.abs() @ W.abs().t()).cpu().double()
+    # 7 * 2^-13 of each group's largest product is at most 2^-10 of its sum of magnitudes
+    near(out, want, want.abs() * half() + size * (2.0 ** -10 + 2 * (K + 8) * U) + least_normal())
