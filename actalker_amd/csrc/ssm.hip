@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256) void causal_conv_step_kernel(const ActhCausalC
 
 template <int VEC, int W>
 void launch_conv(const ActhCausalConvDesc& d, hipStream_t stream) {
-  if (!d.starts && d.nseq == d.T) {
+  if (!d.starts && d.nseq == d.T && d.T <= 65535) {
     const unsigned bx = (unsigned)((d.D + 256 * VEC - 1) / (256 * VEC));
     if ((long long)bx * d.T >= 1024) causal_conv_step_kernel<VEC, W, CSTEP><<<dim3(bx, (unsigned)((d.T + CSTEP - 1) / CSTEP)), 256, 0, stream>>>(d);
     else causal_conv_step_kernel<VEC, W, 1><<<dim3(bx, (unsigned)d.T), 256, 0, stream>>>(d);
@@ -420,6 +420,12 @@ __device__ __forceinline__ float select8(const float* f, int i) {
   return v;
 }
 
+template <int VEC>
+__device__ __forceinline__ uint4 load16_v(const void* p) {
+  if constexpr (VEC == 2) return *reinterpret_cast<const uint4*>(p);
+  else return load16_at(p);
+}
+
 // A wave takes CB channels of a chunk: SPL states a lane, LPC lanes a channel, CPT channels a lane. A tile's time steps
 // (softplus done once, by the staging lane) and inputs dt u sit in LDS as pairs beside the rows of B and C; the output
 // takes the place of the pair that its own lane has just read. The next tile's rows are loaded while this one is
@@ -430,7 +436,8 @@ __device__ __forceinline__ float select8(const float* f, int i) {
 // Bound: the vector units, a row, channel and state taking one exponential (8 clocks a wave) and four operations (4 each):
 // 8192 x 2560 x 16 states 51 us in pass 2 and 43 in pass 1 if nothing else were done; 101 and 80 measured, the rest being
 // the softplus, gate and conversions of the staging lanes and the waves' waits (the units are 75 - 79 % busy).
-template <int SPL, int LPC, int CPT, bool LOCAL, bool VEC>
+// VEC: 2 pieces of 8 channels at multiples of 16 bytes, 1 at any address, 0 groups of fewer than 8 channels
+template <int SPL, int LPC, int CPT, bool LOCAL, int VEC>
 __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p, const Chunks ck) {
   constexpr int CL = 64 / LPC;                     // channels a wave holds at once
   constexpr int CB = CL * CPT;
@@ -459,6 +466,7 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
   const int dsz = p.delta_f32 ? 4 : 2, bsz = p.bc_f32 ? 4 : 2;
   const int fr = lane / C8, fd = min(d0 + lane % C8 * 8, d1 - 8);      // (VEC: a group has 8 channels or more)
   const int back = min(d0 + lane % C8 * 8 - fd, 7);
+  const bool cut = VEC == 1 && ((d1 - d0) & 7) != 0;      // the same for the wave: most have no such piece
   const int gr = lane / NS, gn = lane % NS;
   const bf16_t* at_u = (const bf16_t*)p.u + (long long)(c0 + fr) * p.ldu + fd;
   const char* at_d = (const char*)p.delta + ((long long)(c0 + fr) * p.ld_delta + fd) * dsz;
@@ -473,10 +481,10 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
       for (int k = 0; k < E8; ++k) {
         const int r = fr + 64 / C8 * k;
         if (r < TT && r < left) {
-          pu[k] = load16_at(at_u + (long long)(64 / C8 * k) * p.ldu);
+          pu[k] = load16_v<VEC>(at_u + (long long)(64 / C8 * k) * p.ldu);
           const char* f = at_d + (long long)(64 / C8 * k) * p.ld_delta * dsz;
-          pd[k][0] = load16_at(f);
-          if (p.delta_f32) pd[k][1] = load16_at(f + 16);
+          pd[k][0] = load16_v<VEC>(f);
+          if (p.delta_f32) pd[k][1] = load16_v<VEC>(f + 16);
         }
       }
       at_u += (long long)TT * p.ldu;
@@ -568,18 +576,21 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
       const bool in = r < TT && b0 + r < b1;
       float uf[8], dl[8];
       if constexpr (VEC) {
-        u[k] = down16(pu[k], back);
+        u[k] = pu[k];
+        if (cut) u[k] = down16(u[k], back);
         if (p.delta_f32) {
           dl[0] = __uint_as_float(pd[k][0].x); dl[1] = __uint_as_float(pd[k][0].y);
           dl[2] = __uint_as_float(pd[k][0].z); dl[3] = __uint_as_float(pd[k][0].w);
           dl[4] = __uint_as_float(pd[k][1].x); dl[5] = __uint_as_float(pd[k][1].y);
           dl[6] = __uint_as_float(pd[k][1].z); dl[7] = __uint_as_float(pd[k][1].w);
-          if (back) {
+          if (cut) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) dl[e] = select8(dl, e + back);
           }
         } else {
-          unpack8(down16(pd[k][0], back), dl);
+          uint4 w = pd[k][0];
+          if (cut) w = down16(w, back);
+          unpack8(w, dl);
         }
       } else {
         uint32_t w[4] = {0, 0, 0, 0};
@@ -603,7 +614,7 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
         }
       }
       z[k] = make_uint4(0, 0, 0, 0);
-      if (!LOCAL && p.z && VEC && in && d < d1) z[k] = load16_at((const bf16_t*)p.z + row * p.ldz + fd);
+      if (!LOCAL && p.z && VEC && in && d < d1) z[k] = load16_v<VEC>((const bf16_t*)p.z + row * p.ldz + fd);
     }
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
@@ -632,6 +643,7 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
         if (LOCAL) sum[j] += x.x;
         float y1 = 0.0f;                           // two chains of sums
         y[j] = 0.0f;
+        // (a row's decays all before the first use of one: 86 -> 96 us in pass 1)
 #pragma unroll
         for (int s = 0; s < SPL; ++s) {
           const float a = __builtin_amdgcn_exp2f(x.x * A[j][s]);
@@ -663,7 +675,8 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
         const long long row = b0 + r;
         float y[8], uf[8], zf[8];
         unpack8(u[k], uf);
-        unpack8(down16(z[k], back), zf);
+        if (cut) z[k] = down16(z[k], back);
+        unpack8(z[k], zf);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           y[e] = sx[r][e * C8 + c].x;
@@ -676,7 +689,9 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
             if (d + e < d1) y[e] *= silu16(bf2f(((const bf16_t*)p.z)[row * p.ldz + d + e]));
         }
         bf16_t* o = (bf16_t*)p.y + row * p.ldy + d;
-        if (VEC && back == 0) {
+        if (VEC == 2) {
+          *reinterpret_cast<uint4*>(o) = pack8(y);
+        } else if (VEC == 1 && (!cut || back == 0)) {
           store16_at(o, pack8(y));
         } else {
 #pragma unroll
@@ -910,7 +925,7 @@ Chunks plan(int T, int D, int N, int G, int nseq, int ragged) {
   return c;
 }
 
-template <int SPL, int LPC, int CPT, bool VEC>
+template <int SPL, int LPC, int CPT, int VEC>
 void launch_scan(const ActhSsmScanDesc& d, const Chunks& ck, hipStream_t stream) {
   constexpr int CB = 64 / LPC * CPT;
   const dim3 grid((unsigned)ck.n, (unsigned)(d.G * ((d.D / d.G + CB - 1) / CB)));
@@ -922,7 +937,7 @@ void launch_scan(const ActhSsmScanDesc& d, const Chunks& ck, hipStream_t stream)
   ssm_scan_kernel<SPL, LPC, CPT, false, VEC><<<grid, 64, 0, stream>>>(d, ck);
 }
 
-template <bool VEC>
+template <int VEC>
 void launch_scan_n(const ActhSsmScanDesc& d, const Chunks& ck, hipStream_t stream) {
   if (d.N <= 8) launch_scan<8, 1, 1, VEC>(d, ck, stream);
   else if (scan_small(d.N, d.T, d.D)) launch_scan<8, 2, 1, VEC>(d, ck, stream);
@@ -953,7 +968,6 @@ extern "C" int acth_causal_conv(const ActhCausalConvDesc* d, hipStream_t stream)
     return ACTH_EINVAL;
   if (d->D > (1 << 25)) return ACTH_EINVAL;
   const bool vec = d->D >= 8;
-  if (!d->starts && d->nseq == d->T && d->T > 65535) return ACTH_EINVAL;
   if (vec) {
     if (d->W == 2) launch_conv<8, 2>(*d, stream);
     else if (d->W == 3) launch_conv<8, 3>(*d, stream);
@@ -984,8 +998,7 @@ extern "C" int acth_ssm_scan(const ActhSsmScanDesc* d, hipStream_t stream) {
   if (d->T > 1 && (d->ldu < d->D || d->ld_delta < d->D || d->ldy < d->D || (d->z && d->ldz < d->D) || d->ldb < gn ||
                    d->ldc < gn)) return ACTH_EINVAL;
   if (d->state && d->ld_slot < (long long)d->D * d->N) return ACTH_EINVAL;
-  if (!d->starts && d->nseq == d->T) {
-    if (d->T > 65535) return ACTH_EINVAL;
+  if (!d->starts && d->nseq == d->T && d->T <= 65535) {
     const int bsz = d->bc_f32 ? 4 : 2;             // four values of B and of C in one load
     const bool vbc = (((uintptr_t)d->B | (uintptr_t)d->C | (uintptr_t)(d->ldb * bsz) | (uintptr_t)(d->ldc * bsz)) % (4 * bsz)) == 0;
     if (d->N % 4 == 0 && al16(d->state, d->ld_slot * 4)) {
@@ -1011,9 +1024,11 @@ extern "C" int acth_ssm_scan(const ActhSsmScanDesc* d, hipStream_t stream) {
     ck.kind = (int*)(ck.s + (size_t)ck.places * d->D);
   }
   if (d->G * ((d->D / d->G + 15) / 16) > 65535) return ACTH_EINVAL;
-  const bool vec = d->D / d->G >= 8;
-  if (vec) launch_scan_n<true>(*d, ck, stream);
-  else launch_scan_n<false>(*d, ck, stream);
+  const bool whole = d->D / d->G % 8 == 0 && al16(d->u, d->ldu * 2) && al16(d->delta, d->ld_delta * (d->delta_f32 ? 4 : 2)) &&
+                     al16(d->z, d->ldz * 2) && al16(d->y, d->ldy * 2);
+  if (whole) launch_scan_n<2>(*d, ck, stream);             // 8192 x 5120: 332 us, by the next one 352, 8192 x 5121: 362
+  else if (d->D / d->G >= 8) launch_scan_n<1>(*d, ck, stream);
+  else launch_scan_n<0>(*d, ck, stream);
   ACTH_CHECK_LAUNCH();
   return ACTH_OK;
 }

@@ -632,3 +632,114 @@ def test_gemm_fp8_more_row_blocks_than_a_group(dev):
     want, size = (A @ W.t()).cpu().double(), (A.abs() @ W.abs().t()).cpu().double()
     # 7 * 2^-13 of each group's largest product is at most 2^-10 of its sum of magnitudes
     near(out, want, want.abs() * half() + size * (2.0 ** -10 + 2 * (K + 8) * U) + least_normal())
+
+
+def test_prompts_in_a_graph_with_changing_offsets(dev):
+    """A captured prompt batch: rows, offsets, slots and states change between the replays; eager work runs between."""
+    lay = Layer(dev)
+    T, n = 400, 4
+    x, r = low(T, 256).to(dev), low(T, 256).to(dev)
+    st = torch.tensor([0, 50, 60, 300, 400], dtype=torch.int32, device=dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        lay(x, r, lay.states(n, dev), st)
+    torch.cuda.current_stream().wait_stream(side)
+    gs = lay.states(n, dev)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = lay(x, r, gs, st)
+    es = lay.states(n, dev)
+    for offs in ([0, 50, 60, 300, 400], [0, 0, 399, 400, 400], [0, 400, 400, 400, 400], [0, 100, 200, 300, 400]):
+        x.copy_(low(T, 256))
+        r.copy_(low(T, 256))
+        st.copy_(torch.tensor(offs, dtype=torch.int32))
+        want = [t.clone() for t in lay(x.clone(), r.clone(), es, st.clone())]
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        assert torch.equal(gs[0], es[0]) and torch.equal(gs[1], es[1])
+
+
+def test_calls_without_rows(dev):
+    dt = ops.act_dtype()
+    e, w, A = torch.empty(0, 64, device=dev, dtype=dt), torch.randn(64, 4, device=dev), -torch.rand(64, 16, device=dev)
+    bc = torch.empty(0, 16, device=dev, dtype=dt)
+    kept, h = low(2, 3, 64).to(dev), torch.randn(2, 64, 16, device=dev)
+    c0, h0 = kept.clone(), h.clone()
+    st = torch.zeros(3, dtype=torch.int32, device=dev)
+    assert ops.causal_conv(e, w, starts=st, state=kept).shape == (0, 64)
+    assert ops.ssm_scan(e, e, A, bc, bc, starts=st, state=h).shape == (0, 64)
+    assert ops.causal_conv_step(e, w, state=kept).shape == (0, 64) and ops.ssm_step(e, e, A, bc, bc, state=h).shape == (0, 64)
+    x, b = low(5, 64).to(dev), low(5, 16).to(dev)
+    out = torch.full((5, 64), 3.0, device=dev, dtype=dt)                 # rows, but only empty sequences
+    ops.causal_conv(x, w, starts=st, state=kept, out=out)
+    ops.ssm_scan(x, x, A, b, b, starts=st, state=h, out=out)
+    assert (out == 3.0).all() and torch.equal(kept, c0) and torch.equal(h, h0)
+
+
+def test_output_beside_its_operand(dev):
+    """An output in other columns of an operand's rows is taken, one that shares any is not."""
+    rows = low(40, 192).to(dev)
+    w, st = torch.randn(64, 3, device=dev), torch.tensor([0, 11, 40], dtype=torch.int32, device=dev)
+    want = ops.causal_conv(rows[:, :64].contiguous(), w, starts=st)
+    ops.causal_conv(rows[:, :64], w, starts=st, out=rows[:, 64:128])
+    assert torch.equal(rows[:, 64:128], want)
+    for cols in (slice(32, 96), slice(0, 64)):
+        with pytest.raises(_lib.ActhError):
+            ops.causal_conv(rows[:, :64], w, starts=st, out=rows[:, cols])
+
+
+def test_many_sequences_of_one_row(dev):
+    """More sequences than a launch's second dimension holds."""
+    n, dim = 70001, 8
+    s = scan_case([1], dim, 16, 1, "low")
+    u = low(n, dim).to(dev)
+    args = dict(A=s["A"].to(dev), D=s["D"].to(dev), delta_bias=s["delta_bias"].to(dev))
+    bc, delta = low(n, 32).to(dev), low(n, dim).to(dev)
+    h = torch.randn(n, dim, 16, device=dev)
+    kept = h.clone()
+    y = ops.ssm_step(u, delta, B=bc[:, :16], C=bc[:, 16:], state=kept, **args)
+    w, cst = torch.randn(dim, 4), low(n, 3, dim).to(dev)
+    ckept = cst.clone()
+    c = ops.causal_conv_step(u, w.to(dev), state=ckept)
+    at = torch.tensor([0, 1, 65534, 65535, 65536, n - 1], device=dev)
+    sub, csub = h[at].clone(), cst[at].clone()
+    want = ops.ssm_step(u[at], delta[at], B=bc[at, :16], C=bc[at, 16:], state=sub, **args)
+    # the two kernels add a row's 16 products and the skip in other orders, and each rounds its sum once
+    size = (sub.abs() * bc[at, None, 16:].float().abs()).sum(2) + (args["D"] * u[at].float()).abs()
+    near(y[at], want.double().cpu(), (2 * half() * want.float().abs() + 40 * U * size).double().cpu() + least_normal())
+    near(kept[at], sub.double().cpu(), sub.double().cpu().abs() * 4 * U)
+    assert torch.equal(c[at], ops.causal_conv_step(u[at], w.to(dev), state=csub)) and torch.equal(ckept[at], csub)
+
+
+def test_offsets_past_32_bits(dev, act):
+    """Rows, slots and tiles whose element offsets do not fit 32 bits (one build; the address code is the same)."""
+    if act == "fp16":
+        pytest.skip("the address code does not depend on the activation type")
+    dt = ops.act_dtype()
+    x = torch.zeros(140000, 16384, device=dev, dtype=dt)                  # 2.3e9 elements
+    x[-1] = low(16384).to(dev)
+    q, s = ops.rmsnorm_fp8(x, None)
+    q1, s1 = ops.rmsnorm_fp8(x[-1:].clone(), None)
+    assert torch.equal(q[-1].view(torch.uint8), q1[0].view(torch.uint8)) and torch.equal(s[-1], s1[0])
+    wq, wsc = ops.pack_fp8(torch.randn(64, 16384, device=dev))
+    far, by_itself = ops.gemm_fp8(q, s, wq, wsc)[-1000:].double(), ops.gemm_fp8(q[-1000:].clone(), s[-1000:].contiguous(), wq, wsc).double()
+    assert (far[:-1] == 0).all() and far[-1].abs().max() > 0              # another kernel: other sums, each rounded once
+    assert float((far - by_itself).norm() / by_itself.norm()) < 2 * half()
+    del q, s
+    w = torch.randn(16384, 4, device=dev)
+    st = torch.tensor([0, 7, 139990, 140000], dtype=torch.int32, device=dev)
+    y = ops.causal_conv(x, w, starts=st)
+    assert torch.equal(y[-10:], ops.causal_conv(x[-10:].clone(), w))
+    del x, y
+    dim, N = 2048, 64                                                     # slots of 2^17 floats, 2.6e9 in all
+    pool = torch.empty(20000, dim, N, device=dev)
+    u, b = low(6, dim).to(dev), low(6, N).to(dev)
+    A, start = -torch.rand(dim, N, device=dev), torch.randn(1, dim, N, device=dev)
+    pool[19999] = start[0]
+    one = start.clone()
+    sl = torch.tensor([19999], dtype=torch.int32, device=dev)
+    assert torch.equal(ops.ssm_scan(u, u, A, b, b, state=pool, slots=sl), ops.ssm_scan(u, u, A, b, b, state=one))
+    assert torch.equal(ops.ssm_step(u[:1], u[:1], A, b[:1], b[:1], state=pool, slots=sl), ops.ssm_step(u[:1], u[:1], A, b[:1], b[:1], state=one))
+    assert torch.equal(pool[19999], one[0])
