@@ -691,7 +691,7 @@ def test_output_beside_its_operand(dev):
 
 
 def test_many_sequences_of_one_row(dev):
-    """More sequences than a launch's second dimension holds."""
+    """More sequences than a launch's second dimension could hold."""
     n, dim = 70001, 8
     s = scan_case([1], dim, 16, 1, "low")
     u = low(n, dim).to(dev)
