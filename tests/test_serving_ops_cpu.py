@@ -64,7 +64,7 @@ def test_refusals(lib, fn, cls, good, changes):
 
 def test_scan_workspace(lib):
     size = lib.acth_ssm_scan_workspace_size
-    assert size(100, 64, 16, 1, 1, 0) == 0                                  # one short sequence: one walk
+    assert size(32, 64, 16, 1, 1, 0) == 0                                  # one short sequence: one walk
     need = size(8192, 2560, 16, 1, 1, 0)
     assert need > 0 and need % 4 == 0
     d = made(_lib.SsmScanDesc, **{**SCAN, "T": 8192, "D": 2560, "ldu": 2560, "ld_delta": 2560, "ldy": 2560, "G": 1, "nseq": 1})
