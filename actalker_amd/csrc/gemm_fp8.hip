@@ -511,8 +511,7 @@ extern "C" int acth_gemm_fp8(const ActhGemmFp8Desc* d, hipStream_t stream) {
                    d->K <= 128 * 1024 && 256 * d->as_row < (1 << 28) && (d->K + 127) / 128 * d->as_blk < (1 << 28);
   const long long t256 = (long long)((d->M + 255) / 256) * ((d->N + 255) / 256);
   const long long t128 = (long long)((d->M + 127) / 128) * ((d->N + 127) / 128);
-  if (((long long)d->M + 15) / 16 * (((long long)d->N + 31) / 32) > 0x7fffffff && (d->M <= 32 || t128 <= 40)) return ACTH_EINVAL;
-  if (t128 > 0x7fffffff) return ACTH_EINVAL;
+  if (d->K > (1 << 30) || d->M > (1 << 30) || d->N > (1 << 27) || t128 >= (1 << 23)) return ACTH_EINVAL;      // a launch: less than 2^32 lanes
   // Rounds of the chip: 256 large tiles, or 512 small ones (two blocks a CU), in 1.5 times a small round's time
   // (42 and 27.5 us at K = 2560). 4096 x 2560: 47 against 50 us, 4096 x 5120: 83 against 72, 16384 x 2560 x 5120: 253 against 276.
   const long long r256 = (t256 + 255) / 256, r128 = (t128 + 511) / 512;

@@ -760,7 +760,11 @@ __global__ __launch_bounds__(64) void ssm_carry_kernel(const ActhSsmScanDesc p, 
 #pragma unroll
     for (int v = 0; v < B; ++v) {
       if (k + v >= n) break;
-      h = kind[f][v] ? fmaf(__builtin_amdgcn_exp2f(A * s[f][v]), h, e[f][v]) : e[f][v];
+      // a chunk's decay as two factors, its root: whole, it leaves fp32 where its product with h does not, and h = 0
+      // stays 0 under any growth
+      const float root = __builtin_amdgcn_exp2f(0.5f * A * s[f][v]);
+      const float grown = h == 0.0f ? 0.0f : root * (root * h);
+      h = kind[f][v] ? e[f][v] + grown : e[f][v];
       if (kind[f][v]) ck.h[(long long)(k + v) * dn + i] = h;
     }
   };

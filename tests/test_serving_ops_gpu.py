@@ -743,3 +743,29 @@ def test_offsets_past_32_bits(dev, act):
     assert torch.equal(ops.ssm_scan(u, u, A, b, b, state=pool, slots=sl), ops.ssm_scan(u, u, A, b, b, state=one))
     assert torch.equal(ops.ssm_step(u[:1], u[:1], A, b[:1], b[:1], state=pool, slots=sl), ops.ssm_step(u[:1], u[:1], A, b[:1], b[:1], state=one))
     assert torch.equal(pool[19999], one[0])
+
+
+def test_chunks_whose_decay_leaves_fp32(dev):
+    """A long row of time steps over which exp(A sum dt) overflows or underflows while every state stays in range."""
+    s = scan_case([400], 16, 16, 1, "float")
+    s["delta"] = torch.zeros(400, 16)
+    s["delta"][32:48] = 1.0
+    s["delta"][300:] = 0.1
+    s["A"][:] = -1.0
+    s["A"][2], s["A"][3], s["A"][4], s["A"][5] = 6.0, 6.0, -6.0, 9.0
+    s["u"][:, 2:6] = 0
+    s["state"][0, 2], s["state"][0, 3], s["state"][0, 4], s["state"][0, 5] = 1e-30, 0.0, 1e30, 0.0
+    s["delta"][300:, 2:4] = 0.0
+    s["u"][395:, 5] = 1.0                                    # nothing, growth past every number, then something
+    s["delta"][300:395, 5] = 2.0
+    s["z"] = torch.ones_like(s["z"])
+    s["C"] = s["C"] * 1e-20                                  # outputs inside 16 bits' range
+    s["D"] = torch.zeros(16)
+    for starts in (None, torch.tensor([0, 400], dtype=torch.int32, device=dev)):
+        args = (s["u"], s["delta"], s["A"], s["B"], s["C"], s["D"], s["z"], None, False)
+        y, tol, new, ntol = scan_ref(*args, [0, 400], s["state"], [False])
+        kept = s["state"].to(dev)
+        out = ops.ssm_scan(**to(dev, s, "u", "delta", "A", "B", "C", "D", "z"), softplus=False, starts=starts, state=kept)
+        keep = [c for c in range(16) if c != 4] if ops.act_dtype() is torch.float16 else list(range(16))      # 1e30 * 1e-20
+        near(out[:, keep], y[:, keep], tol[:, keep], "y")
+        near(kept, new, ntol, "state")
