@@ -63,6 +63,18 @@ __device__ __forceinline__ bool seq_kept(const P& p, const Seq& q) {        // d
   return p.state && q.slot >= 0 && !(p.fresh && p.fresh[q.i]);
 }
 
+// the sequence behind q that may hold row t or a later one: not one by one over empty ones, of which a padded batch has
+// many in one place (a search from the front, which offsets out of order cannot lead back)
+template <class P>
+__device__ __forceinline__ Seq seq_next(const P& p, const Seq& q, int t) {
+  Seq n = seq_of(p, q.i + 1);
+  if (p.starts && n.i < p.nseq && n.e <= t) {
+    const Seq f = seq_find(p, t);
+    if (f.i > n.i) n = f;
+  }
+  return n;
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 // x / (1 + exp(-x)) with the one-step reciprocal: within 4 roundings of 2^-24, for 16-bit outputs
@@ -198,7 +210,7 @@ __global__ __launch_bounds__(64) void causal_conv_kernel(const ActhCausalConvDes
     if (q.i < 0 || q.i >= p.nseq || q.e <= t) {                  // rows that no sequence holds, or an empty sequence
       if (q.i >= p.nseq) return;
       if (q.i < 0) t = max(t, q.e);
-      q = seq_of(p, q.i + 1);
+      q = seq_next(p, q, t);
       if (q.i < p.nseq && q.s > t) t = q.s;
       continue;
     }
@@ -256,7 +268,7 @@ __global__ __launch_bounds__(64) void causal_conv_kernel(const ActhCausalConvDes
       }
     }
     t = max(t, q.e);
-    q = seq_of(p, q.i + 1);
+    q = seq_next(p, q, t);
     if (q.i < p.nseq && q.s > t) t = q.s;
   }
 }

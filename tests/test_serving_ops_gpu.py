@@ -769,3 +769,16 @@ def test_chunks_whose_decay_leaves_fp32(dev):
         keep = [c for c in range(16) if c != 4] if ops.act_dtype() is torch.float16 else list(range(16))      # 1e30 * 1e-20
         near(out[:, keep], y[:, keep], tol[:, keep], "y")
         near(kept, new, ntol, "state")
+
+
+def test_padded_batch_inside_a_tile(dev):
+    """Many empty sequences in one place, in the middle of the rows, with sequences behind them."""
+    lens = [5] + [0] * 700 + [9, 0, 0, 20] + [0] * 300
+    n, D = len(lens), 64
+    cuts = cuts_of(lens)
+    x, w, bias, st = low(cuts[-1] + 3, D), torch.randn(D, 4), torch.randn(D), low(n, 3, D)
+    y, tol, new = conv_ref(x, w, bias, cuts, st, [False] * n, True)
+    kept, out = st.to(dev), torch.full(x.shape, 3.0, device=dev, dtype=ops.act_dtype())
+    ops.causal_conv(x.to(dev), w.to(dev), bias.to(dev), starts=torch.tensor(cuts, dtype=torch.int32, device=dev), state=kept, out=out)
+    near(out[:cuts[-1]], y[:cuts[-1]], tol[:cuts[-1]])
+    assert (out[cuts[-1]:] == 3.0).all() and torch.equal(kept.cpu(), new.to(ops.act_dtype()))
