@@ -323,12 +323,36 @@ __global__ __launch_bounds__(256) void causal_conv_step_kernel(const ActhCausalC
   }
 }
 
+// A launch holds less than 2^32 lanes: rows that blocks of 256 lanes, `per_row` of them a row, may take in one
+constexpr int LAUNCH = 1 << 24;
+int launch_rows(long long per_row) { return (int)((LAUNCH - 1) / per_row) & ~7; }
+
+// rows [t0, t0 + n) of a step, which is one sequence a row
+template <class P>
+P step_rows(P d, int t0, int n) {
+  d.T = d.nseq = n;
+  if (d.fresh) d.fresh += t0;
+  if (d.slots) {
+    d.slots += t0;
+  } else if (d.state) {
+    d.state = (decltype(d.state))((char*)d.state + t0 * d.ld_slot * (std::is_same<P, ActhSsmScanDesc>::value ? 4 : 2));
+    d.nslots -= t0;
+  }
+  return d;
+}
+
 template <int VEC, int W>
 void launch_conv(const ActhCausalConvDesc& d, hipStream_t stream) {
   if (!d.starts && d.nseq == d.T) {
     const unsigned bx = (unsigned)((d.D + 256 * VEC - 1) / (256 * VEC));
-    if ((long long)bx * d.T >= 1024) causal_conv_step_kernel<VEC, W, CSTEP><<<(unsigned)((d.T + CSTEP - 1) / CSTEP) * bx, 256, 0, stream>>>(d);
-    else causal_conv_step_kernel<VEC, W, 1><<<(unsigned)d.T * bx, 256, 0, stream>>>(d);
+    const int rows = launch_rows(bx);
+    for (int t0 = 0; t0 < d.T; t0 += rows) {
+      ActhCausalConvDesc s = step_rows(d, t0, d.T - t0 < rows ? d.T - t0 : rows);
+      s.x = (const bf16_t*)d.x + t0 * d.ldx;
+      s.y = (bf16_t*)d.y + t0 * d.ldy;
+      if ((long long)bx * s.T >= 1024) causal_conv_step_kernel<VEC, W, CSTEP><<<(unsigned)((s.T + CSTEP - 1) / CSTEP) * bx, 256, 0, stream>>>(s);
+      else causal_conv_step_kernel<VEC, W, 1><<<(unsigned)s.T * bx, 256, 0, stream>>>(s);
+    }
   } else {
     const dim3 grid((unsigned)((d.T + CT - 1) / CT), (unsigned)((d.D + 64 * VEC - 1) / (64 * VEC)));
     causal_conv_kernel<VEC, W><<<grid, 64, 0, stream>>>(d);
@@ -903,8 +927,18 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(const ActhSsmScanDesc p) 
 
 template <int VN, int LPC, int SEQS, bool VBC>
 void launch_step2(const ActhSsmScanDesc& d, hipStream_t stream) {
-  const unsigned grid = (unsigned)((d.T + SEQS - 1) / SEQS) * (unsigned)((d.D * LPC + 255) / 256);
-  ssm_step_kernel<VN, LPC, SEQS, VBC><<<grid, 256, 0, stream>>>(d);
+  const unsigned bx = (unsigned)((d.D * LPC + 255) / 256);
+  const int rows = launch_rows(bx), bsz = d.bc_f32 ? 4 : 2;
+  for (int t0 = 0; t0 < d.T; t0 += rows) {
+    ActhSsmScanDesc s = step_rows(d, t0, d.T - t0 < rows ? d.T - t0 : rows);
+    s.u = (const bf16_t*)d.u + t0 * d.ldu;
+    s.delta = (const char*)d.delta + t0 * d.ld_delta * (d.delta_f32 ? 4 : 2);
+    s.B = (const char*)d.B + t0 * d.ldb * bsz;
+    s.C = (const char*)d.C + t0 * d.ldc * bsz;
+    if (d.z) s.z = (const bf16_t*)d.z + t0 * d.ldz;
+    s.y = (bf16_t*)d.y + t0 * d.ldy;
+    ssm_step_kernel<VN, LPC, SEQS, VBC><<<(unsigned)((s.T + SEQS - 1) / SEQS) * bx, 256, 0, stream>>>(s);
+  }
 }
 
 // several sequences a lane once there are enough lanes to fill the chip without it
@@ -999,7 +1033,6 @@ extern "C" int acth_causal_conv(const ActhCausalConvDesc* d, hipStream_t stream)
   if (!seqs_ok(d->T, d->nseq, d->starts, d->slots, d->state, d->nslots)) return ACTH_EINVAL;
   if ((d->T > 1 && (d->ldx < d->D || d->ldy < d->D)) || (d->state && d->ld_slot < (long long)(d->W - 1) * d->D))
     return ACTH_EINVAL;
-  if (!d->starts && d->nseq == d->T && (long long)d->T * ((d->D + 255) / 256) > 0x7fffffffLL) return ACTH_EINVAL;
   const bool vec = d->D >= 8;
   if (vec) {
     if (d->W == 2) launch_conv<8, 2>(*d, stream);
@@ -1032,7 +1065,6 @@ extern "C" int acth_ssm_scan(const ActhSsmScanDesc* d, hipStream_t stream) {
                    d->ldc < gn)) return ACTH_EINVAL;
   if (d->state && d->ld_slot < (long long)d->D * d->N) return ACTH_EINVAL;
   if (!d->starts && d->nseq == d->T) {
-    if ((long long)d->T * ((d->D + 3) / 4) > 0x7fffffffLL) return ACTH_EINVAL;      // blocks of a launch
     const int bsz = d->bc_f32 ? 4 : 2;             // four values of B and of C in one load
     const bool vbc = (((uintptr_t)d->B | (uintptr_t)d->C | (uintptr_t)(d->ldb * bsz) | (uintptr_t)(d->ldc * bsz)) % (4 * bsz)) == 0;
     if (d->N % 4 == 0 && al16(d->state, d->ld_slot * 4)) {
@@ -1057,7 +1089,7 @@ extern "C" int acth_ssm_scan(const ActhSsmScanDesc* d, hipStream_t stream) {
     ck.s = ck.h + (size_t)ck.places * d->D * d->N;
     ck.kind = (int*)(ck.s + (size_t)ck.places * d->D);
   }
-  if (d->G * ((d->D / d->G + 15) / 16) > 65535) return ACTH_EINVAL;
+  if (d->G * ((d->D / d->G + 15) / 16) > 65535 || ck.n >= 4 * LAUNCH) return ACTH_EINVAL;      // blocks of a launch, 64 lanes each
   const bool whole = d->D / d->G % 8 == 0 && al16(d->u, d->ldu * 2) && al16(d->delta, d->ld_delta * (d->delta_f32 ? 4 : 2)) &&
                      al16(d->z, d->ldz * 2) && al16(d->y, d->ldy * 2);
   if (whole) launch_scan_n<2>(*d, ck, stream);             // 8192 x 5120: 332 us, by the next one 352, 8192 x 5121: 362

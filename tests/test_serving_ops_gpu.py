@@ -782,3 +782,42 @@ def test_padded_batch_inside_a_tile(dev):
     ops.causal_conv(x.to(dev), w.to(dev), bias.to(dev), starts=torch.tensor(cuts, dtype=torch.int32, device=dev), state=kept, out=out)
     near(out[:cuts[-1]], y[:cuts[-1]], tol[:cuts[-1]])
     assert (out[cuts[-1]:] == 3.0).all() and torch.equal(kept.cpu(), new.to(ops.act_dtype()))
+
+
+def test_more_rows_than_a_launch(dev, act):
+    """Norms and steps of so many rows that one launch could not hold a block each (the split does not depend on the type)."""
+    if act == "fp16":
+        pytest.skip("the launches do not depend on the activation type")
+    n = (1 << 24) + 37
+    dt = ops.act_dtype()
+    at = torch.tensor([0, 1, (1 << 24) - 9, (1 << 24) - 8, (1 << 24) - 7, (1 << 24) - 1, 1 << 24, n - 1], device=dev)
+    x, r = torch.randn(n, 3, device=dev).to(dt), torch.randn(n, 3, device=dev)
+    (y, s), (y1, s1) = ops.rmsnorm(x, None, residual=r), ops.rmsnorm(x[at], None, residual=r[at])
+    assert torch.equal(y[at], y1) and torch.equal(s, x.float() + r)
+    q, sc = ops.quant_fp8(x)
+    q1, sc1 = ops.quant_fp8(x[at])
+    assert torch.equal(q[at].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(sc[at], sc1)
+    del y, s, q, sc, r
+    u, w = x[:, :1].contiguous(), torch.tensor([[0.5, 2.0]], device=dev)
+    st = torch.randn(n, 1, 1, device=dev).to(dt)
+    kept = st.clone()
+    y = ops.causal_conv_step(u, w, state=kept, silu=False)                # 16-bit sums of two exact products
+    assert torch.equal(kept[:, 0], u) and torch.equal(y, (0.5 * st[:, 0].float() + 2.0 * u.float()).to(dt))
+    perm = (n - 1 - torch.arange(n, device=dev)).int()
+    fresh = torch.zeros(n, dtype=torch.bool, device=dev)
+    fresh[-1] = True
+    kept = st.clone()
+    y = ops.causal_conv_step(u, w, state=kept, slots=perm, fresh=fresh, silu=False)
+    old = st.flip(0)[:, 0].float()
+    old[-1] = 0
+    assert torch.equal(kept.flip(0)[:, 0], u) and torch.equal(y, (0.5 * old + 2.0 * u.float()).to(dt))
+    A = torch.zeros(1, 1, device=dev)                                     # no decay: h + delta u B, powers of two apart
+    b = torch.ones(n, 1, device=dev)
+    delta = torch.full((n, 1), 0.5, device=dev)
+    h = torch.randint(-8, 9, (n, 1, 1), device=dev).float()
+    ui = torch.randint(-8, 9, (n, 1), device=dev).to(dt)
+    for slots in (None, perm):
+        kept = h.clone()
+        y = ops.ssm_step(ui, delta, A, b, b, state=kept, slots=slots, softplus=False)
+        want = (h if slots is None else h.flip(0))[:, 0] + 0.5 * ui.float()
+        assert torch.equal(kept[:, 0] if slots is None else kept.flip(0)[:, 0], want) and torch.equal(y.float(), want)
