@@ -114,9 +114,9 @@ __device__ __forceinline__ int4 load16_any(const uint8_t* row, int k, int K) {
 // Bound: 8192^3 takes 531 us (2070 TFLOP/s; the card's library reaches 2690 with one scale for a whole operand, 1260 in 16
 // bits). The matrix unit is busy 47 % of the time and the vector unit, with the scales' multiply-adds, 38 %, at the
 // 1.9 GHz that the card holds under this load; 17 % of the time goes to the LDS-DMA beside the products and 5 % to the
-// multiply-adds (both timed by leaving them out of a copy). Then whole rounds of 256 tiles: 16384 x 2560 is 2.5 of them
-// and costs 3 (253 us, 1700 TFLOP/s). A ring of three 256 x 128 stages, which would be five full rounds there, moves twice
-// the bytes a product through L2 and took 275 us.
+// multiply-adds (both timed by leaving them out of a copy). Then rounds of 256 tiles: 16384 x 2560 is 2.5 of them, the last
+// taken as a round of half tiles, at 0.65 of a round's time (238 us, 1800 TFLOP/s at K = 5120; whole tiles 251; a ring of
+// three 256 x 128 stages, five full rounds there, moves twice the bytes a product through L2 and took 275).
 template <int BM, int BN>
 struct Tile {
   static constexpr int WC = BN / 64, WR = 8 / WC;              // waves along n and m
@@ -151,13 +151,17 @@ struct Stage {
   }
 };
 
-// tiles: each XCD takes a contiguous run; inside it gm row blocks x all column blocks, rows fastest, so the tiles that an
-// XCD holds at once share their rows of A and W in its L2
+// workgroup b of nwg takes this place of the tiles' order: each XCD a contiguous run
+__device__ __forceinline__ int place_of(int b, int nwg) {
+  const int xcd = b & 7, qn = nwg >> 3, rn = nwg & 7;
+  return (xcd < rn ? xcd * (qn + 1) : rn * (qn + 1) + (xcd - rn) * qn) + (b >> 3);
+}
+
+// the tiles' order: gm row blocks x all column blocks, rows fastest, so the tiles that an XCD holds at once share their
+// rows of A and W in its L2
 template <int BM, int BN>
-__device__ __forceinline__ void tile_of(const ActhGemmFp8Desc& p, int gm, int& m0, int& n0) {
-  const int ntn = (p.N + BN - 1) / BN, ntm = (p.M + BM - 1) / BM, nwg = gridDim.x;
-  const int xcd = blockIdx.x & 7, qn = nwg >> 3, rn = nwg & 7;
-  const int lin = (xcd < rn ? xcd * (qn + 1) : rn * (qn + 1) + (xcd - rn) * qn) + (blockIdx.x >> 3);
+__device__ __forceinline__ void tile_at(const ActhGemmFp8Desc& p, int gm, int lin, int& m0, int& n0) {
+  const int ntn = (p.N + BN - 1) / BN, ntm = (p.M + BM - 1) / BM;
   const int grp = lin / (gm * ntn), mg0 = grp * gm, gcur = min(gm, ntm - mg0), rest = lin - grp * gm * ntn;
   n0 = rest / gcur * BN;
   m0 = (mg0 + rest % gcur) * BM;
@@ -205,21 +209,20 @@ __device__ __forceinline__ void step(const char* __restrict__ rd, char* __restri
   }
 }
 
+constexpr int MAXKB = 1024;
+template <int BM, int BN>                          // two stages (rows of A, of W, and the row scales), W's scales
+constexpr int lds_bytes() { return 2 * (Tile<BM, BN>::STAGE + BM * 4) + MAXKB * (BN / 128) * 4; }
+
 template <int BM, int BN, bool WIDE>
-__global__ __launch_bounds__(512, BM * BN > 128 * 128 || WIDE ? 2 : 4) void gemm_fp8_kernel(const ActhGemmFp8Desc p, int gm, int vec_out) {
+__device__ __forceinline__ void gemm_fp8_tile(const ActhGemmFp8Desc& p, int m0, int n0, int vec_out, char* smem) {
   using T = Tile<BM, BN>;
-  constexpr int STAGE = T::STAGE + BM * 4;                      // a block's rows of A, of W, and the row scales
-  constexpr int MAXKB = 1024;
-  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE + MAXKB * (BN / 128) * 4];
+  constexpr int STAGE = T::STAGE + BM * 4;
   float* const s_ws = reinterpret_cast<float*>(smem + 2 * STAGE);             // [kb][BN / 128]
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wave % T::WR, wc = wave / T::WR;
   const int r16 = lane & 15, g = lane >> 4;
-
-  int m0, n0;
-  tile_of<BM, BN>(p, gm, m0, n0);
   const int nkb = (p.K + 127) / 128;
 
   const int mrows = min(BM, p.M - m0), nrows = min(BN, p.N - n0);
@@ -271,6 +274,28 @@ __global__ __launch_bounds__(512, BM * BN > 128 * 128 || WIDE ? 2 : 4) void gemm
       finish4(p, m0 + (wr * T::TM + i) * 16 + r16, n0 + wc * 64 + j * 16 + g * 4, acc[i][j], vec_out);
 }
 
+template <bool WIDE>
+__global__ __launch_bounds__(512, WIDE ? 2 : 4) void gemm_fp8_kernel(const ActhGemmFp8Desc p, int gm, int vec_out) {
+  __shared__ __attribute__((aligned(16))) char smem[lds_bytes<128, 128>()];
+  int m0, n0;
+  tile_at<128, 128>(p, gm, place_of(blockIdx.x, gridDim.x), m0, n0);
+  gemm_fp8_tile<128, 128, WIDE>(p, m0, n0, vec_out, smem);
+}
+
+// 256 x 256 tiles, the first `whole` of them by a workgroup each, the others in halves of 128 columns
+__global__ __launch_bounds__(512, 2) void gemm_fp8_large_kernel(const ActhGemmFp8Desc p, int gm, int whole, int vec_out) {
+  __shared__ __attribute__((aligned(16))) char smem[lds_bytes<256, 256>()];
+  int m0, n0;
+  if ((int)blockIdx.x < whole) {
+    tile_at<256, 256>(p, gm, place_of(blockIdx.x, whole), m0, n0);
+    gemm_fp8_tile<256, 256, false>(p, m0, n0, vec_out, smem);
+  } else {
+    const int at = place_of(blockIdx.x - whole, gridDim.x - whole);
+    tile_at<256, 256>(p, gm, whole + (at >> 1), m0, n0);
+    n0 += (at & 1) * 128;
+    if (n0 < p.N) gemm_fp8_tile<256, 128, false>(p, m0, n0, vec_out, smem);
+  }
+}
 
 // The 128 x 128 tile for operands that the LDS-DMA cannot take (rows at any address, a K that ends inside 16 bytes, very
 // long rows): the next block goes through registers, loaded before this one's products and written to LDS after them.
@@ -288,7 +313,7 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_any_kernel(const ActhGemmFp8D
   const int wr = wave % T::WR, wc = wave / T::WR;
   const int r16 = lane & 15, g = lane >> 4;
   int m0, n0;
-  tile_of<BM, BN>(p, gm, m0, n0);
+  tile_at<BM, BN>(p, gm, place_of(blockIdx.x, gridDim.x), m0, n0);
   const int nkb = (p.K + 127) / 128;
   const int chunk = (lane & 7) ^ (lane >> 3);
   const uint8_t* ar[T::AP];
@@ -351,9 +376,8 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_any_kernel(const ActhGemmFp8D
       finish4(p, m0 + (wr * T::TM + i) * 16 + r16, n0 + wc * 64 + j * 16 + g * 4, acc[i][j], vec_out);
 }
 
-template __global__ void gemm_fp8_kernel<256, 256, false>(const ActhGemmFp8Desc, int, int);
-template __global__ void gemm_fp8_kernel<128, 128, false>(const ActhGemmFp8Desc, int, int);
-template __global__ void gemm_fp8_kernel<128, 128, true>(const ActhGemmFp8Desc, int, int);
+template __global__ void gemm_fp8_kernel<false>(const ActhGemmFp8Desc, int, int);
+template __global__ void gemm_fp8_kernel<true>(const ActhGemmFp8Desc, int, int);
 template __global__ void gemm_fp8_any_kernel<false>(const ActhGemmFp8Desc, int, int);
 template __global__ void gemm_fp8_any_kernel<true>(const ActhGemmFp8Desc, int, int);
 
@@ -512,9 +536,12 @@ extern "C" int acth_gemm_fp8(const ActhGemmFp8Desc* d, hipStream_t stream) {
   const long long t256 = (long long)((d->M + 255) / 256) * ((d->N + 255) / 256);
   const long long t128 = (long long)((d->M + 127) / 128) * ((d->N + 127) / 128);
   if (d->K > (1 << 30) || d->M > (1 << 30) || d->N > (1 << 27) || t128 >= (1 << 23)) return ACTH_EINVAL;      // a launch: less than 2^32 lanes
-  // Rounds of the chip: 256 large tiles, or 512 small ones (two blocks a CU), in 1.5 times a small round's time
-  // (42 and 27.5 us at K = 2560). 4096 x 2560: 47 against 50 us, 4096 x 5120: 83 against 72, 16384 x 2560 x 5120: 253 against 276.
-  const long long r256 = (t256 + 255) / 256, r128 = (t128 + 511) / 512;
+  // Rounds of the chip: 256 large tiles in 1.5 times the time of 512 small ones (two blocks a CU; 42 and 27.5 us at K =
+  // 2560). A last round of at most 128 large tiles is taken in halves, in a small round's time. Large against small:
+  // 4096 x 2560 44 against 47 us, 4096 x 5120 72 against 73, 4096 x 2048 29.5 against 29.1, 9216 x 2560 76 against 83.
+  // Halves against whole tiles: 16384 x 2560 x 5120 238 against 251, 9216 x 2560 76 against 88.
+  const int rest = (int)(t256 % 256), halves = rest <= 128 ? rest : 0;
+  const long long large = t256 / 256 * 3 + (halves ? 2 : rest ? 3 : 0), small = (t128 + 511) / 512 * 2;
   if (d->M <= 32 || t128 <= 40) {                // 256 x 2560 x 2560: 14.6 against 16.2 us, 512 rows: 27.5 against 16.7
     if (dma) d->out_f32 ? launch_few<true, true>(*d, vec_out, stream) : launch_few<false, true>(*d, vec_out, stream);
     else d->out_f32 ? launch_few<true, false>(*d, vec_out, stream) : launch_few<false, false>(*d, vec_out, stream);
@@ -522,12 +549,12 @@ extern "C" int acth_gemm_fp8(const ActhGemmFp8Desc* d, hipStream_t stream) {
     if (d->out_f32) gemm_fp8_any_kernel<true><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
     else gemm_fp8_any_kernel<false><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
   } else if (d->out_f32) {
-    gemm_fp8_kernel<128, 128, true><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
-  } else if (3 * r256 < 2 * r128) {
+    gemm_fp8_kernel<true><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
+  } else if (large < small) {
     // row blocks side by side: 4, 8, 16, 32: 450, 480, 480, 513 us at 16384 x 10240 x 2560, 249, 256, 256, 257 at 16384 x 2560 x 5120
-    gemm_fp8_kernel<256, 256, false><<<(unsigned)t256, 512, 0, stream>>>(*d, 4, vec_out);
+    gemm_fp8_large_kernel<<<(unsigned)(t256 + halves), 512, 0, stream>>>(*d, 4, (int)(t256 - halves), vec_out);
   } else {
-    gemm_fp8_kernel<128, 128, false><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
+    gemm_fp8_kernel<false><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
   }
   ACTH_CHECK_LAUNCH();
   return ACTH_OK;
