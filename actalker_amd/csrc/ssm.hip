@@ -83,12 +83,11 @@ __device__ __forceinline__ float silu16(float x) {
 }
 
 // ------------------------------------------------------------------------------------------------ convolution
-// VEC channels a lane (8: one 16-byte load a row, from any address; 1: fewer than 8 channels), a wave 64 x VEC channels of 16 rows. The
-// rows of a tile are loaded before the first is used; the W - 1 rows in front of it are read again (3 of 16, from L2).
+// VEC channels a lane (8: one 16-byte load a row, from any address; 1: fewer than 8 channels), a wave 64 x VEC channels of CT rows. The
+// rows of a tile are loaded before the first is used; the W - 1 rows in front of it are read again (3 beside 16, from L2).
 // The tile that holds a sequence's first row also takes the rows that reach back into the kept inputs and writes the
 // new ones, so one lane both reads and writes each kept value. Bound: HBM bandwidth (32768 x 5120 x 4 taps, 24 sequences:
 // 154 us, 4.4 TB/s; 8 or 32 rows a tile: 168, 154; channels that fill no 8: 190).
-constexpr int CT = 16;
 
 template <int VEC>
 __device__ __forceinline__ void load_c(const bf16_t* p, float* f) {
@@ -177,7 +176,7 @@ struct ConvLane {
   }
 };
 
-template <int VEC, int W>
+template <int VEC, int W, int CT>
 __global__ __launch_bounds__(64) void causal_conv_kernel(const ActhCausalConvDesc p) {
   const int t0 = blockIdx.x * CT, t1 = min(t0 + CT, p.T);
   const int d_ = (blockIdx.y * 64 + threadIdx.x) * VEC;
@@ -354,8 +353,14 @@ void launch_conv(const ActhCausalConvDesc& d, hipStream_t stream) {
       else causal_conv_step_kernel<VEC, W, 1><<<(unsigned)s.T * bx, 256, 0, stream>>>(s);
     }
   } else {
-    const dim3 grid((unsigned)((d.T + CT - 1) / CT), (unsigned)((d.D + 64 * VEC - 1) / (64 * VEC)));
-    causal_conv_kernel<VEC, W><<<grid, 64, 0, stream>>>(d);
+    const unsigned by = (unsigned)((d.D + 64 * VEC - 1) / (64 * VEC));
+    const auto tiles = [&](int rows) { return dim3((unsigned)((d.T + rows - 1) / rows), by); };
+    // Tiles of 16 rows that leave SIMDs idle (there are 1024) are cut: 4, 8, 16 rows, a call in a graph: 300 x 640 6.2, 7.0,
+    // 10.1 us, 1000 x 1306 7.8, 9.2, 12.0; 1000 x 5120 11.8, 10.1, 11.2, 4000 x 2560 16.5, 14.2, 16.6; 8000 x 2560 24.0, 22.1, 20.2.
+    const long long waves = (long long)tiles(16).x * by;
+    if (waves < 512) causal_conv_kernel<VEC, W, 4><<<tiles(4), 64, 0, stream>>>(d);
+    else if (waves < 2048) causal_conv_kernel<VEC, W, 8><<<tiles(8), 64, 0, stream>>>(d);
+    else causal_conv_kernel<VEC, W, 16><<<tiles(16), 64, 0, stream>>>(d);
   }
 }
 

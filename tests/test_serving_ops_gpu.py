@@ -821,3 +821,19 @@ def test_more_rows_than_a_launch(dev, act):
         y = ops.ssm_step(ui, delta, A, b, b, state=kept, slots=slots, softplus=False)
         want = (h if slots is None else h.flip(0))[:, 0] + 0.5 * ui.float()
         assert torch.equal(kept[:, 0] if slots is None else kept.flip(0)[:, 0], want) and torch.equal(y.float(), want)
+
+
+@pytest.mark.parametrize("W", [2, 3, 4])
+@pytest.mark.parametrize("T,D", [(600, 8192), (2300, 8195)])
+def test_causal_conv_of_every_tile(dev, T, D, W):
+    """Rows and channels enough for tiles of 8 and of 16 rows: each channel as in a call of a few channels, bit for bit."""
+    cuts = [0, 1, 1, 3, 7, 100, 115, 116, 118, 333, 333, T - 5]
+    n = len(cuts) - 1
+    x, w, bias, st = low(T, D).to(dev), torch.randn(D, W).to(dev), torch.randn(D).to(dev), low(n, W - 1, D).to(dev)
+    args = dict(starts=torch.tensor(cuts, dtype=torch.int32, device=dev), fresh=(torch.rand(n) < 0.3).to(dev))
+    kept, out = st.clone(), torch.full_like(x, 3.0)
+    ops.causal_conv(x, w, bias, state=kept, out=out, **args)
+    for at in (slice(0, 40), slice(4000, 4040), slice(D - 40, D)):
+        k, o = st[:, :, at].contiguous(), torch.full_like(x[:, at], 3.0)
+        ops.causal_conv(x[:, at].contiguous(), w[at].contiguous(), bias[at].contiguous(), state=k, out=o, **args)
+        assert torch.equal(out[:, at], o) and torch.equal(kept[:, :, at], k)
