@@ -975,7 +975,7 @@ Chunks plan(int T, int D, int N, int G, int nseq, int ragged) {
   const int cb = scan_cb(N, T, D);
   const long long waves = (long long)G * ((D / G + cb - 1) / cb);
   const int L = ragged ? T : T / nseq;             // the longest sequence there can be
-  long long n = 3072 / waves;                      // chunks of all rows
+  long long n = 3 * 1024 / waves;                  // chunks of all rows
   if (!ragged) n /= nseq;                          // of one sequence
   if (n < 1) n = 1;
   long long len = (L + n - 1) / n;
