@@ -101,15 +101,15 @@ __device__ __forceinline__ float gelu_erf(float x) {
   return 0.5f * x * (1.0f + erf_as(x * 0.70710678118654752f));
 }
 
-// Two GELUs in packed f32x2 arithmetic, no transcendental: erf(z) = z * P(z^2) on z clamped to
-// [-3.3, 3.3] (erf(3.3) = 1 - 3.1e-6), P a degree-11 Chebyshev fit in z^2 evaluated by Horner with
-// v_pk_fma_f32. |erf error| <= 4.3e-5 in fp32 (|GELU error| <= 1.0e-4 at |x| ~ 4, i.e. < 1 % of a
+// Two GELUs side by side (f32x2, two scalar instructions each: the build uses no packed fp32), no transcendental: erf(z) = z * P(z^2) on z clamped to
+// [-3.3, 3.3] (erf(3.3) = 1 - 3.1e-6), P a degree-11 Chebyshev fit in z^2 evaluated by
+// Horner. |erf error| <= 4.3e-5 in fp32 (|GELU error| <= 1.0e-4 at |x| ~ 4, i.e. < 1 % of a
 // bf16 ulp there), against two quarter-rate transcendentals + 7 scalar FMAs per value in gelu_erf:
 // the GEGLU epilogue of the K = 320 / 640 GEMMs is VALU-bound on this math.
 typedef float float2_pk __attribute__((ext_vector_type(2)));
 
 // The same GELU from the degree-8 erf fit of ffn.hip (erf(g / sqrt 2) = gc * Q(gc^2), gc = g clamped to
-// +-2.95 sqrt 2, |GELU error| <= 7.4e-5): 12 packed ops per pair instead of 16.
+// +-2.95 sqrt 2, |GELU error| <= 7.4e-5): 12 operations instead of 16.
 __device__ __forceinline__ float2_pk gelu_pk8(float2_pk x) {
   constexpr float c[9] = {0.7977727652f, -0.1326450109f, 0.01961599849f, -0.002216302557f, 1.874310692e-04f,
                           -1.138649350e-05f, 4.631291688e-07f, -1.116308557e-08f, 1.195545885e-10f};
