@@ -10,9 +10,11 @@
 // Precision. The 8-bit matrix instructions add products in groups of 8 consecutive k and drop what lies below 2^-13 of
 // the group's largest product (toward zero; measured on the card lane by lane, the same for the 32-deep form), which
 // costs up to 7 * 2^-13 of a group's largest product and in practice 2e-6 (signed) to 3e-6 (positive data) of the sum
-// of magnitudes: far below a 16-bit output's half step of 2^-9 or 2^-12. fp32 outputs would show it (1.8e-5 of their
-// norm), so those products go through the 16-bit matrix instructions instead, where e4m3 values are exact and the same
-// sums are off by 1e-9 to 1e-8; that unit runs at half the rate.
+// of magnitudes. Tiles of many rows with 16-bit outputs, which the matrix rate bounds, take that: 2.7e-5 of the output's
+// norm beside the 1.66e-3 (bf16) or 2.1e-4 (fp16) of its own rounding (16384 x 2560 x 5120: distance from the 64-bit
+// result 1.65572e-3, of that result rounded 1.65566e-3; fp16 2.0750e-4 and 2.0700e-4). fp32 outputs would show it
+// (1.8e-5 of their norm), and few rows, which the weights' bytes bound, gain little by it: those products go through
+// the 16-bit matrix instructions, where e4m3 values are exact and the same sums are off by 1e-9 to 1e-8, at half the rate.
 #include "gemm_common.h"
 
 namespace {
@@ -386,12 +388,14 @@ namespace {
 // ---- few rows: a tile of 16 MT x 16 NT, its k blocks dealt to the eight waves in turn (few rows make few tiles, so the
 // long axis has to fill the chip), each wave's fragments straight from memory: no wave waits for another until the
 // partial sums meet in LDS, in a fixed order. A lane loads two 16-byte pieces of its row, k [16 g, 16 g + 16) and 64
-// further. Rows behind the last read it again.
-// Bound: the weights' bytes and the latency of the two or three blocks each wave takes (1 x 10240 x 2560: 8.5 us, 3.1 TB/s;
-// 1 x 2560 x 2560: 5.6 us; two or four blocks' loads at once changed neither), then L2, which serves A and W to every
-// tile: larger row counts take larger tiles.
-template <int MT, int NT, bool WIDE, bool ALIGNED>
-__global__ __launch_bounds__(512, MT * NT > 8 || (MT * NT == 8 && (WIDE || !ALIGNED)) ? 2 : 4) void gemm_fp8_few_kernel(const ActhGemmFp8Desc p, int vec_out) {
+// further. Rows behind the last read it again. The sums go through the 16-bit unit, exact to fp32's roundings; the 8-bit one
+// would save 4 to 20 % where a wave takes three blocks or more (32 columns a workgroup: 1 x 2560 x 2560 5.5 against 6.5 us,
+// 1 x 5120 x 640 3.6 and 3.7).
+// Bound: the weights' bytes and the latency of the two or three blocks each wave takes (1 x 10240 x 2560 from memory: 10.7
+// us, 2.5 TB/s; 1 x 2560 x 2560: 6.6 us; two or four blocks' loads at once changed neither), then L2, which serves A and W
+// to every tile: larger row counts take larger tiles.
+template <int MT, int NT, bool ALIGNED>
+__global__ __launch_bounds__(512, MT * NT >= 8 ? 2 : 4) void gemm_fp8_few_kernel(const ActhGemmFp8Desc p, int vec_out) {
   constexpr int TILES = MT * NT;
   __shared__ __attribute__((aligned(16))) f32x4_t red[4][TILES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -459,26 +463,17 @@ __global__ __launch_bounds__(512, MT * NT > 8 || (MT * NT == 8 && (WIDE || !ALIG
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) d[i][j] = (f32x4_t){0, 0, 0, 0};
-    if constexpr (WIDE) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        bf16x8_t wa[MT], ww[NT];
+    for (int c = 0; c < 4; ++c) {
+      bf16x8_t wa[MT], ww[NT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) wa[i] = wide8(fa[i][c >> 1][(c & 1) * 2], fa[i][c >> 1][(c & 1) * 2 + 1]);
+      for (int i = 0; i < MT; ++i) wa[i] = wide8(fa[i][c >> 1][(c & 1) * 2], fa[i][c >> 1][(c & 1) * 2 + 1]);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) ww[j] = wide8(fw[j][c >> 1][(c & 1) * 2], fw[j][c >> 1][(c & 1) * 2 + 1]);
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int j = 0; j < NT; ++j) d[i][j] = mfma16x16x32(ww[j], wa[i], d[i][j]);
-      }
-    } else {
+      for (int j = 0; j < NT; ++j) ww[j] = wide8(fw[j][c >> 1][(c & 1) * 2], fw[j][c >> 1][(c & 1) * 2 + 1]);
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-          d[i][j] = mfma8(__builtin_shufflevector(fw[j][0], fw[j][1], 0, 1, 2, 3, 4, 5, 6, 7),
-                          __builtin_shufflevector(fa[i][0], fa[i][1], 0, 1, 2, 3, 4, 5, 6, 7), d[i][j]);
+        for (int j = 0; j < NT; ++j) d[i][j] = mfma16x16x32(ww[j], wa[i], d[i][j]);
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
@@ -507,16 +502,19 @@ __global__ __launch_bounds__(512, MT * NT > 8 || (MT * NT == 8 && (WIDE || !ALIG
   }
 }
 
-template <bool WIDE, bool ALIGNED>
+template <bool ALIGNED>
 void launch_few(const ActhGemmFp8Desc& d, int vec_out, hipStream_t stream) {
   auto tiles = [&](int mt, int nt) { return (unsigned)(((d.M + 16 * mt - 1) / (16 * mt)) * ((d.N + 16 * nt - 1) / (16 * nt))); };
+  // 32 columns a workgroup against 64, up to 16 rows (weights from memory, a call in a graph): 1 x 2560 x 2560 6.6 against
+  // 9.8 us, 1 x 10240 x 2560 10.7 against 11.6, 1 x 16384 x 5120 19.9 against 23.2; 16 rows 7.4 against 11.0, 13.4 against
+  // 12.7, 24.8 against 24.2. 32 rows a tile while they leave CUs free: 128 x 2560 x 2560 12.1 against 15.5 us of 64 rows,
+  // 128 x 5120 x 2560 23.8 against 17.4.
   if (d.M <= 16) {
-    if (tiles(1, 4) >= 128) gemm_fp8_few_kernel<1, 4, WIDE, ALIGNED><<<tiles(1, 4), 512, 0, stream>>>(d, vec_out);
-    else gemm_fp8_few_kernel<1, 2, WIDE, ALIGNED><<<tiles(1, 2), 512, 0, stream>>>(d, vec_out);
+    gemm_fp8_few_kernel<1, 2, ALIGNED><<<tiles(1, 2), 512, 0, stream>>>(d, vec_out);
   } else if (d.M <= 32 || tiles(4, 4) < 128) {
-    gemm_fp8_few_kernel<2, 4, WIDE, ALIGNED><<<tiles(2, 4), 512, 0, stream>>>(d, vec_out);
+    gemm_fp8_few_kernel<2, 4, ALIGNED><<<tiles(2, 4), 512, 0, stream>>>(d, vec_out);
   } else {
-    gemm_fp8_few_kernel<4, 4, WIDE, ALIGNED><<<tiles(4, 4), 512, 0, stream>>>(d, vec_out);
+    gemm_fp8_few_kernel<4, 4, ALIGNED><<<tiles(4, 4), 512, 0, stream>>>(d, vec_out);
   }
 }
 
@@ -542,9 +540,10 @@ extern "C" int acth_gemm_fp8(const ActhGemmFp8Desc* d, hipStream_t stream) {
   // Halves against whole tiles: 16384 x 2560 x 5120 238 against 251, 9216 x 2560 76 against 88.
   const int rest = (int)(t256 % 256), halves = rest <= 128 ? rest : 0;
   const long long large = t256 / 256 * 3 + (halves ? 2 : rest ? 3 : 0), small = (t128 + 511) / 512 * 2;
-  if (d->M <= 32 || t128 <= 40) {                // 256 x 2560 x 2560: 14.6 against 16.2 us, 512 rows: 27.5 against 16.7
-    if (dma) d->out_f32 ? launch_few<true, true>(*d, vec_out, stream) : launch_few<false, true>(*d, vec_out, stream);
-    else d->out_f32 ? launch_few<true, false>(*d, vec_out, stream) : launch_few<false, false>(*d, vec_out, stream);
+  // (weights from memory) 256 x 2560 x 2560 15.7 against 22.3 us, 512 rows 28.4 against 24.3; 1024 x 640 x 2560 14.7 against 19.7
+  if (d->M <= 32 || t128 <= 40) {
+    if (dma) launch_few<true>(*d, vec_out, stream);
+    else launch_few<false>(*d, vec_out, stream);
   } else if (!dma) {
     if (d->out_f32) gemm_fp8_any_kernel<true><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
     else gemm_fp8_any_kernel<false><<<(unsigned)t128, 512, 0, stream>>>(*d, 16, vec_out);
