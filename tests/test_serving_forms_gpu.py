@@ -1,12 +1,15 @@
 """GPU: the serving operators' kernels at the sizes where each of their forms is chosen, against 64 bits or exact values,
 and what a call owes the framework around it. Tolerances as in test_serving_ops_gpu.py."""
+import math
+
 import pytest
 import torch
 
 from actalker_amd import ops
-from tests.test_serving_ops_gpu import _seed, act      # noqa: F401 (fixtures)
+from tests.test_serving_ops_gpu import _seed, act, half, least_normal, low      # noqa: F401
 
 pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
 
 
 # ------------------------------------------------------------------------------------------ product
@@ -25,3 +28,62 @@ def test_gemm_fp8_few_rows_keep_small_products(dev, M, N, K):
     for f32 in (False, True):
         out = ops.gemm_fp8(a.to(ops.FP8).to(dev), s.to(dev), w.to(ops.FP8).to(dev), ws.to(dev), out_f32=f32)
         assert torch.equal(out.float().cpu(), want)
+
+
+def product_and_size(a, s, w, ws, bias=None, res=None):
+    """The product in 64 bits on the device, and the sum of the magnitudes that enter it."""
+    big = lambda t, c, r: t.double() * c.double().repeat_interleave(r, 0)[:t.shape[0]].repeat_interleave(128, 1)[:, :t.shape[1]]   # noqa: E731
+    A, W = big(a.float(), s, 1), big(w.float(), ws, 128).t().contiguous()
+    want, size = A @ W, A.abs() @ W.abs()
+    for more in (bias, res):
+        if more is not None:
+            want, size = want + more.double(), size + more.double().abs()
+    return want, size
+
+
+# a product of K > 0 in one call of each form: (M, N, K, operands inside wider rows)
+FORMS = [(1, 10250, 2560, False), (16, 8203, 517, True), (16, 8200, 520, False), (33, 640, 1306, False), (1000, 512, 517, True),
+         (1000, 512, 512, False), (1100, 1030, 1306, True), (1100, 1030, 1296, False),
+         (4096 - 13, 2560 - 24, 656, False),       # 160 large tiles, none of them halved
+         (9216 - 37, 2560 - 21, 1296, False)]      # 360 large tiles, the last 104 in halves
+
+
+@pytest.mark.parametrize("M,N,K,inside", FORMS)
+@pytest.mark.parametrize("more", ["none", "bias_res", "f32"])
+def test_gemm_fp8_forms(dev, M, N, K, inside, more):
+    """Element by element: 7 * 2^-13 of each group's largest product, the most that the 8-bit unit may drop, is at most
+    2^-10 of the sum of magnitudes. In the norm: what it drops of a product has the product's sign and is at most 2^-13 of
+    its group's largest, uniformly spread, so over random signs at most sqrt(7 / 3) 2^-13 of the product's norm, which
+    adds to the outputs' own rounding as squares do."""
+    a, w = low(M, K).to(dev), (torch.randn(N, K) / math.sqrt(K)).to(dev)
+    (q, s), (wq, wsc) = ops.quant_fp8(a), ops.pack_fp8(w)
+    if inside:
+        pad = lambda t, l, r: torch.nn.functional.pad(t.view(torch.uint8), (l, r), value=0x7e).view(ops.FP8)[:, l:l + K]   # noqa: E731
+        q, wq = pad(q, 3, 8), pad(wq, 5, 2)
+    bias = torch.randn(N, device=dev) if more == "bias_res" else None
+    res = low(M, N).to(dev) if more == "bias_res" else None
+    out = ops.gemm_fp8(q, s, wq, wsc, bias=bias, residual=res, out_f32=more == "f32")
+    want, size = product_and_size(q, s, wq, wsc, bias, res)
+    err = (out.double() - want).abs()
+    if more == "f32":
+        assert (err <= size * (K + 8) * U).all()
+        return
+    assert (err <= size * (2.0 ** -10 + (K + 8) * U) + want.abs() * half() + least_normal()).all()
+    product = want if res is None else product_and_size(q, s, wq, wsc)[0]
+    own = want.to(out.dtype).double() - want
+    assert float(err.square().sum()) <= 1.002 * float(own.square().sum()) + 7 / 3 * 2.0 ** -26 * float(product.square().sum())
+
+
+@pytest.mark.parametrize("M,N,K", [(2, 40, 256), (300, 640, 256), (1100, 1030, 256), (4096, 2560, 256)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_gemm_fp8_a_code_that_is_no_number(dev, M, N, K, f32):
+    """A NaN code reaches its row, or its column, and nothing else."""
+    q, s = ops.quant_fp8(low(M, K).to(dev))
+    w, ws = ops.pack_fp8(torch.randn(N, K, device=dev))
+    good = ops.gemm_fp8(q, s, w, ws, out_f32=f32)
+    q.view(torch.uint8)[M // 2, 200] = 0x7f
+    w.view(torch.uint8)[N - 3, 5] = 0xff
+    bad = ops.gemm_fp8(q, s, w, ws, out_f32=f32)
+    hit = torch.zeros(M, N, dtype=torch.bool, device=dev)
+    hit[M // 2], hit[:, N - 3] = True, True
+    assert torch.equal(torch.isnan(bad), hit) and torch.equal(bad[~hit], good[~hit])
