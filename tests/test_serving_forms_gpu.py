@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from actalker_amd import ops
-from tests.test_serving_ops_gpu import _seed, act, half, least_normal, low      # noqa: F401
+from tests.test_serving_ops_gpu import (IN, _seed, act, cuts_of, half, least_normal, low, near, scan_case, scan_ref,      # noqa: F401
+                                        to)
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -87,3 +88,36 @@ def test_gemm_fp8_a_code_that_is_no_number(dev, M, N, K, f32):
     hit = torch.zeros(M, N, dtype=torch.bool, device=dev)
     hit[M // 2], hit[:, N - 3] = True, True
     assert torch.equal(torch.isnan(bad), hit) and torch.equal(bad[~hit], good[~hit])
+
+
+# ------------------------------------------------------------------------------------------ scan and steps
+def channels(s, at, G):
+    """The call's operands for the channels `at` of one group alone, on the CPU."""
+    dim, N = s["A"].shape
+    g = at.start // (dim // G)
+    assert (at.stop - 1) // (dim // G) == g
+    cut = {k: s[k][..., at].contiguous() for k in ("u", "delta", "z", "D", "delta_bias")}
+    return dict(cut, A=s["A"][at], B=s["B"][:, g * N:(g + 1) * N], C=s["C"][:, g * N:(g + 1) * N], state=s["state"][:, at])
+
+
+@pytest.mark.parametrize("dim,N,G,kind", [(2048, 16, 1, "low"), (2051, 16, 1, "float"), (2051, 12, 1, "low"), (4104, 16, 2, "float"),
+                                          (2048, 12, 512, "low")])
+@pytest.mark.parametrize("lens", [[2900, 0, 1, 1299], [4200], [1400] * 3], ids=str)
+def test_ssm_scan_of_wide_layers(dev, dim, N, G, kind, lens):
+    """Rows and channels enough for one lane a channel: chunks with and without a carry, a last piece of channels that is
+    whole, cut or shorter than 8 (groups of 4), the first, middle and last channels of the first and last group."""
+    s = scan_case(lens, dim, N, G, kind, extra=3 if len(set(lens)) > 1 else 0)
+    T, cuts, n = s["u"].shape[0], cuts_of(lens), len(lens)
+    assert T // 64 * (-(-dim // 64)) >= 2048
+    fresh = torch.rand(n) < 0.3
+    kept, out = s["state"].to(dev), torch.full((T, dim), 3.0, device=dev, dtype=ops.act_dtype())
+    how = dict(nb=n) if T == cuts[-1] and len(set(lens)) == 1 else dict(starts=torch.tensor(cuts, dtype=torch.int32, device=dev))
+    ops.ssm_scan(**to(dev, s, *IN), state=kept, fresh=fresh.to(dev), out=out, **how)
+    dg = dim // G
+    first = [slice(0, 4)] if dg < 12 else [slice(0, 9), slice(59, 70), slice(dg - 12, dg)]
+    for at in first + [slice(dim - dg + a.start, dim - dg + a.stop) for a in first] * (G > 1):
+        c = channels(s, at, G)
+        y, tol, new, ntol = scan_ref(*(c[k] for k in IN), True, cuts, c["state"], fresh)
+        near(out[:cuts[-1], at], y[:cuts[-1]], tol[:cuts[-1]], f"y {at}")
+        near(kept[:, at], new, ntol, f"state {at}")
+    assert (out[cuts[-1]:] == 3.0).all()
