@@ -121,3 +121,30 @@ def test_ssm_scan_of_wide_layers(dev, dim, N, G, kind, lens):
         near(out[:cuts[-1], at], y[:cuts[-1]], tol[:cuts[-1]], f"y {at}")
         near(kept[:, at], new, ntol, f"state {at}")
     assert (out[cuts[-1]:] == 3.0).all()
+
+
+@pytest.mark.parametrize("n,dim,N,G", [(257, 2560, 16, 1), (257, 2560, 5, 1), (129, 1284, 24, 2), (131, 640, 64, 1), (257, 1024, 8, 1), (12001, 12, 16, 1)])
+@pytest.mark.parametrize("beside", [False, True])
+def test_ssm_step_of_many_sequences(dev, n, dim, N, G, beside):
+    """Sequences enough that a lane takes two, an odd number of them, some without a place and some that start from zeros;
+    B and C at whole or odd addresses."""
+    s = scan_case([1] * n, dim, N, G, "low")
+    slots, fresh = torch.randperm(n + 3)[:n].to(torch.int32), torch.rand(n) < 0.2
+    slots[5], slots[n - 1] = -1, n + 3                 # the first and the second of a pair
+    live = [i for i in range(n) if 0 <= slots[i] < n + 3]
+    at = slots[live].long()
+    pool = torch.randn(n + 3, dim, N)
+    state = torch.zeros(n, dim, N)
+    state[live] = pool[at]
+    y, tol, new, ntol = scan_ref(*(s[k] for k in IN), True, list(range(n + 1)), state, fresh)
+    kept, out = pool.to(dev), torch.full((n, dim), 3.0, device=dev, dtype=ops.act_dtype())
+    args = to(dev, s, *IN)
+    if beside:
+        rows = torch.cat([s["B"][:, :1], s["B"], s["C"], s["C"][:, :1]], 1).to(dev)
+        args["B"], args["C"] = rows[:, 1:1 + G * N], rows[:, 1 + G * N:1 + 2 * G * N]
+    ops.ssm_step(**args, state=kept, slots=slots.to(dev), fresh=fresh.to(dev), out=out)
+    near(out[live], y[live], tol[live], "y")
+    near(kept[at], new[live], ntol[live], "state")
+    dead = [i for i in range(n) if i not in live]
+    rest = [i for i in range(n + 3) if i not in set(at.tolist())]
+    assert (out[dead] == 3.0).all() and torch.equal(kept.cpu()[rest], pool[rest])
