@@ -16,6 +16,7 @@ import threading
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -859,7 +860,8 @@ _CHECK_ARGS = os.environ.get("ACTH_CHECK_ARGS", "0") == "1"
 
 
 def _served(what: str, *tensors) -> int:
-    """Index of the one device of the operands that are given; refuses CPU tensors, several devices and autograd."""
+    """Index of the one device of the operands that are given; refuses CPU tensors, several devices and operands that
+    are being differentiated."""
     idx = tensors[0].get_device()
     for t in tensors:
         if t is not None and (idx < 0 or t.get_device() != idx):
@@ -867,11 +869,21 @@ def _served(what: str, *tensors) -> int:
             if not t.is_cuda:
                 raise _lib.ActhError(f"{what}: expected a device tensor, got {t.device}")
             raise _lib.ActhError(f"{what}: operands on {tensors[0].device} and {t.device}")
+    _not_differentiated(what, tensors)
+    return idx
+
+
+def _not_differentiated(what: str, tensors):
+    """Refuses operands that reverse-mode autograd records, and ones that carry a forward-mode tangent (which
+    torch.no_grad() keeps): a kernel given their addresses would drop it in silence."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise _lib.ActhError(f"{what} has no backward: call it under torch.no_grad() or detach its operands")
-    return idx
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise _lib.ActhError(f"{what} has no forward-mode derivative: unpack its operands' primals first")
 
 
 # One call of these operators is a few microseconds of GPU time at small sizes, so the host path is kept short: the

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from actalker_amd import ops
+from actalker_amd import _lib, ops
 from tests.test_serving_ops_gpu import (IN, _seed, act, cuts_of, half, least_normal, low, near, scan_case, scan_ref,      # noqa: F401
                                         to)
 
@@ -148,3 +148,39 @@ def test_ssm_step_of_many_sequences(dev, n, dim, N, G, beside):
     dead = [i for i in range(n) if i not in live]
     rest = [i for i in range(n + 3) if i not in set(at.tolist())]
     assert (out[dead] == 3.0).all() and torch.equal(kept.cpu()[rest], pool[rest])
+
+
+# ------------------------------------------------------------------------------------------ around a call
+def calls(dev, n=4, d=64):
+    """Every entry point as (name, operands by name, call of them); the states and outputs are among the operands."""
+    dt = ops.act_dtype()
+    q, s = ops.quant_fp8(low(n, d).to(dev))
+    w, ws = ops.pack_fp8(torch.randn(48, d, device=dev))
+    x = lambda: low(n, d).to(dev)                                                                     # noqa: E731
+    scan = lambda **k: dict(u=x(), delta=x(), A=-torch.rand(d, 16, device=dev), B=low(n, 16).to(dev), C=low(n, 16).to(dev),   # noqa: E731
+                            z=x(), state=torch.zeros(n, d, 16, device=dev), out=x(), **k)
+    conv = lambda: dict(x=x(), w=torch.randn(d, 4, device=dev), bias=torch.randn(d, device=dev),      # noqa: E731
+                        state=torch.zeros(n, 3, d, device=dev, dtype=dt), out=x())
+    st = torch.tensor([0, 1, n], dtype=torch.int32, device=dev)
+    return [
+        ("rmsnorm", dict(x=x(), gamma=torch.ones(d, device=dev), residual=x(), sum_out=x(), out=x()), ops.rmsnorm),
+        ("rmsnorm_fp8", dict(x=x(), gamma=torch.ones(d, device=dev), residual=torch.randn(n, d, device=dev),
+                             sum_out=torch.zeros(n, d, device=dev)), ops.rmsnorm_fp8),
+        ("quant_fp8", dict(x=x()), ops.quant_fp8),
+        ("gemm_fp8", dict(a=q, a_scale=s, w=w, w_scale=ws, bias=torch.ones(48, device=dev), residual=low(n, 48).to(dev),
+                          out=torch.empty(n, 48, device=dev, dtype=dt)), ops.gemm_fp8),
+        ("causal_conv", dict(conv(), starts=st), ops.causal_conv), ("causal_conv_step", conv(), ops.causal_conv_step),
+        ("ssm_scan", scan(starts=st), ops.ssm_scan), ("ssm_step", scan(), ops.ssm_step),
+    ]
+
+
+def test_operands_with_a_tangent_are_refused(dev):
+    from torch.autograd import forward_ad
+    for name, args, f in calls(dev):
+        f(**args)
+        with forward_ad.dual_level():
+            f(**args)
+            for k, t in args.items():
+                if t.dtype in (torch.float32, ops.act_dtype()):
+                    with torch.no_grad(), pytest.raises(_lib.ActhError, match="forward-mode"):
+                        f(**dict(args, **{k: forward_ad.make_dual(t, torch.ones_like(t))}))

@@ -95,3 +95,19 @@ def test_pack_fp8(N, K):
     assert (err <= torch.maximum(w.double().abs() * 2.0 ** -4, big * 2.0 ** -10) * (1 + 2.0 ** -20)).all()
     z, sz = ops.pack_fp8(torch.zeros(3, 5))
     assert (z.float() == 0).all() and (sz > 0).all()
+
+
+def test_operands_with_a_tangent_are_refused():
+    """Forward-mode tangents outlive torch.no_grad(); offsets, codes and absent operands carry none."""
+    from torch.autograd import forward_ad
+    x, ids, q = torch.randn(3, 4), torch.zeros(4, dtype=torch.int32), torch.zeros(3, 4, dtype=ops.FP8)
+    with forward_ad.dual_level():
+        ops._not_differentiated("op", (x, None, ids, q))
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(_lib.ActhError, match="forward-mode"):
+                ops._not_differentiated("op", (ids, None, d))
+        ops._not_differentiated("op", (forward_ad.unpack_dual(d).primal,))
+    ops._not_differentiated("op", (x, ids))
+    with pytest.raises(_lib.ActhError, match="no backward"):
+        ops._not_differentiated("op", (x, x.clone().requires_grad_()))
