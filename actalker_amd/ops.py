@@ -899,6 +899,12 @@ def _launch_on(idx: int, fn, d, name: str):
         _lib.check(rc, name)
 
 
+def _written(*tensors):
+    """Counts up the versions of the caller's tensors that a launch has written, as torch's in-place operations do: a
+    graph that saved one refuses its backward, and what is cached by version (masks, packed weights) is made again."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+
+
 _SERVE_LIBS = {}
 
 
@@ -963,6 +969,7 @@ def _rmsnorm(name, x, gamma, eps, residual, sum_out, out, eight, norm):
     dev = x.device
     ldx = _mat(x, shape, adt, name + " x")
     res, ldres, res_f32, ldsum, scale, ld_out = None, 0, 0, 0, None, 0
+    given = sum_out, out
     if residual is not None:
         kind = residual.dtype
         if kind is not torch.float32 and kind is not adt:
@@ -997,6 +1004,8 @@ def _rmsnorm(name, x, gamma, eps, residual, sum_out, out, eight, norm):
                          None if scale is None else scale.data_ptr(), 1, M, M, C)
     if M:
         _launch_on(idx, _serve_lib(adt).acth_rmsnorm, d, "acth_rmsnorm")
+        if given[0] is not None or given[1] is not None:
+            _written(*given)
     if eight:
         return (out, scale) if sum_out is None else (out, scale, sum_out)
     return out if sum_out is None else (out, sum_out)
@@ -1066,6 +1075,7 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: t
         if t.dtype is not torch.float32 or t.shape != shape:
             raise _lib.ActhError(f"gemm_fp8 {what}: expected fp32 of shape {shape}, got {tuple(t.shape)} {t.dtype}")
     kind = torch.float32 if out_f32 else adt
+    given = out
     if out is None:
         out, ldc = torch.empty_strided((M, N), (N, 1), device=a.device, dtype=kind), N
     else:
@@ -1081,6 +1091,8 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: t
                          out.data_ptr(), ldc, out_f32, M, N, K)
     if M:
         _launch_on(idx, _serve_lib(adt).acth_gemm_fp8, d, "acth_gemm_fp8")
+        if given is not None:
+            _written(given)
     return out
 
 
@@ -1153,6 +1165,7 @@ def causal_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] =
     ld_slot = 0
     if state is not None:
         ld_slot = _state(state, W - 1, D, adt, name + " state")
+    given = out
     if out is None:
         out, ldy = torch.empty_strided(shape, (D, 1), device=x.device, dtype=adt), D
     else:
@@ -1164,6 +1177,8 @@ def causal_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] =
                             p_starts, p_slots, p_fresh, out.data_ptr(), ldy, T, D, W, n, nslots, silu)
     if T:
         _launch_on(idx, _serve_lib(adt).acth_causal_conv, d, "acth_causal_conv")
+        if state is not None or given is not None:
+            _written(state, given)
     return out
 
 
@@ -1207,6 +1222,7 @@ def ssm_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Ten
     ld_slot = 0
     if state is not None:
         ld_slot = _state(state, dim, N, torch.float32, name + " state")
+    given = out
     if out is None:
         out, ldy = torch.empty_strided(shape, (dim, 1), device=u.device, dtype=adt), dim
     else:
@@ -1229,6 +1245,8 @@ def ssm_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Ten
                          out.data_ptr(), ldy, T, dim, N, G, n, nslots, softplus, None if ws is None else ws.data_ptr(), need)
     if T:
         _launch_on(idx, lib.acth_ssm_scan, d, "acth_ssm_scan")
+        if state is not None or given is not None:
+            _written(state, given)
     del ws
     return out
 

@@ -184,3 +184,25 @@ def test_operands_with_a_tangent_are_refused(dev):
                 if t.dtype in (torch.float32, ops.act_dtype()):
                     with torch.no_grad(), pytest.raises(_lib.ActhError, match="forward-mode"):
                         f(**dict(args, **{k: forward_ad.make_dual(t, torch.ones_like(t))}))
+
+
+def test_written_tensors_count_up_their_version(dev):
+    """States and given outputs, and nothing else; so a backward that needs a state's old values refuses to run."""
+    for name, args, f in calls(dev):
+        before = {k: t._version for k, t in args.items()}
+        f(**args)
+        for k, t in args.items():
+            assert (t._version > before[k]) == (k in ("sum_out", "out", "state")), (name, k)
+    _, args, f = calls(dev)[-1]
+    scale = torch.ones(1, device=dev, requires_grad=True)
+    y = (scale * args["state"]).sum()
+    with torch.no_grad():
+        f(**args)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        f(**dict(args, state=torch.zeros_like(args["state"])))
+    empty = dict(args, **{k: args[k][:0] for k in ("u", "delta", "B", "C", "z", "out")})
+    version = args["state"]._version
+    f(**empty)
+    assert args["state"]._version == version
