@@ -1102,12 +1102,12 @@ def _sequences(name, T, nb, starts, slots, fresh, state):
         if starts.dtype is not torch.int32 or starts.dim() != 1 or starts.numel() < 2 or not starts.is_contiguous():
             raise _lib.ActhError(f"{name} starts: expected contiguous int32 row offsets, one more than sequences")
         nb = starts.numel() - 1
-    elif nb < 1 or T % nb:
+    elif nb < 0 or (T % nb if nb else T):
         raise _lib.ActhError(f"{name}: {T} rows are not {nb} equal sequences")
     nslots = 0
     if state is not None:
         nslots = state.shape[0]
-        if nslots < (nb if slots is None else 1):
+        if nslots < (nb if slots is None else min(nb, 1)):
             raise _lib.ActhError(f"{name}: {nslots} states for {nb} sequences")
     if slots is not None:
         if state is None:
@@ -1186,7 +1186,7 @@ def causal_conv_step(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tens
                      slots: Optional[torch.Tensor] = None, fresh: Optional[torch.Tensor] = None, silu: bool = True,
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`causal_conv` of one new token of each sequence: x (n, D), row i belongs to sequence i."""
-    return causal_conv(x, w, bias, nb=max(1, x.shape[0]), state=state, slots=slots, fresh=fresh, silu=silu, out=out)
+    return causal_conv(x, w, bias, nb=x.shape[0], state=state, slots=slots, fresh=fresh, silu=silu, out=out)
 
 
 def ssm_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
@@ -1256,5 +1256,5 @@ def ssm_step(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Ten
              delta_bias: Optional[torch.Tensor] = None, softplus: bool = True, slots: Optional[torch.Tensor] = None,
              fresh: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`ssm_scan` of one new token of each sequence: u (n, d), row i belongs to sequence i."""
-    return ssm_scan(u, delta, A, B, C, D=D, z=z, delta_bias=delta_bias, softplus=softplus, nb=max(1, u.shape[0]),
+    return ssm_scan(u, delta, A, B, C, D=D, z=z, delta_bias=delta_bias, softplus=softplus, nb=u.shape[0],
                     state=state, slots=slots, fresh=fresh, out=out)

@@ -206,3 +206,14 @@ def test_written_tensors_count_up_their_version(dev):
     version = args["state"]._version
     f(**empty)
     assert args["state"]._version == version
+
+
+def test_steps_of_a_batch_that_has_run_empty(dev):
+    for name, args, f in calls(dev):
+        if name.endswith("_step"):
+            kept = args["state"].fill_(2.0)
+            rows = {k: t if k in ("w", "bias", "A", "state") else t[:0] for k, t in args.items()}
+            none = torch.empty(0, dtype=torch.int32, device=dev)
+            assert f(**rows, slots=none, fresh=none.bool()).shape == (0, 64)
+            assert f(**dict(rows, state=kept[:0]), slots=none).shape == (0, 64)
+            assert (kept == 2.0).all()

@@ -111,3 +111,17 @@ def test_operands_with_a_tangent_are_refused():
     ops._not_differentiated("op", (x, ids))
     with pytest.raises(_lib.ActhError, match="no backward"):
         ops._not_differentiated("op", (x, x.clone().requires_grad_()))
+
+
+def test_sequences_of_no_rows():
+    """A batch that has run empty: no rows, no sequences, so no slots either, in a pool of any size."""
+    none = torch.zeros(0, dtype=torch.int32)
+    for pool in (0, 3):
+        got = ops._sequences("op", 0, 0, None, none, none.bool(), torch.zeros(pool, 2, 4))
+        assert got[3:] == (0, pool)
+    assert ops._sequences("op", 0, 1, None, None, None, None)[3] == 1        # one empty sequence
+    for T, nb in ((5, 0), (0, -1), (5, -5), (5, 2)):
+        with pytest.raises(_lib.ActhError):
+            ops._sequences("op", T, nb, None, None, None, None)
+    with pytest.raises(_lib.ActhError):
+        ops._sequences("op", 0, 0, None, torch.zeros(1, dtype=torch.int32), None, torch.zeros(2, 2, 4))
