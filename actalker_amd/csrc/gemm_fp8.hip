@@ -534,10 +534,11 @@ extern "C" int acth_gemm_fp8(const ActhGemmFp8Desc* d, hipStream_t stream) {
   const long long t256 = (long long)((d->M + 255) / 256) * ((d->N + 255) / 256);
   const long long t128 = (long long)((d->M + 127) / 128) * ((d->N + 127) / 128);
   if (d->K > (1 << 30) || d->M > (1 << 30) || d->N > (1 << 27) || t128 >= (1 << 23)) return ACTH_EINVAL;      // a launch: less than 2^32 lanes
-  // Rounds of the chip: 256 large tiles in 1.5 times the time of 512 small ones (two blocks a CU; 42 and 27.5 us at K =
-  // 2560). A last round of at most 128 large tiles is taken in halves, in a small round's time. Large against small:
-  // 4096 x 2560 44 against 47 us, 4096 x 5120 72 against 73, 4096 x 2048 29.5 against 29.1, 9216 x 2560 76 against 83.
-  // Halves against whole tiles: 16384 x 2560 x 5120 238 against 251, 9216 x 2560 76 against 88.
+  // Rounds of the chip: 256 large tiles in 1.5 times the time of 512 small ones (two blocks a CU). A last round of at most
+  // 128 large tiles is taken in halves, in a small round's time. Large against small, in a graph: 4096 x 2560 of K = 640,
+  // 2560, 5120, 10240: 21.3 against 19.8 us, 43.4 and 47.2, 72 and 82, 128 and 149; 4096 x 5120: 31.4 and 30.2, 71 and 73, 121 and
+  // 129, 224 and 240; 9216 x 2560: 32.4 and 34.4, 73 and 81, 130 and 147, 236 and 274. Halves against whole tiles: 16384 x
+  // 2560: 52 and 59, 121 and 132, 215 and 235, 396 and 415. So the rule loses 8 % at most, where K is short.
   const int rest = (int)(t256 % 256), halves = rest <= 128 ? rest : 0;
   const long long large = t256 / 256 * 3 + (halves ? 2 : rest ? 3 : 0), small = (t128 + 511) / 512 * 2;
   // (weights from memory) 256 x 2560 x 2560 15.7 against 22.3 us, 512 rows 28.4 against 24.3; 1024 x 640 x 2560 14.7 against 19.7

@@ -77,7 +77,10 @@ __device__ __forceinline__ Seq seq_next(const P& p, const Seq& q, int t) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// x / (1 + exp(-x)) with the one-step reciprocal: within 4 roundings of 2^-24, for 16-bit outputs
+// x / (1 + exp(-x)) with the one-step reciprocal, for 16-bit outputs. The exponential and the reciprocal are off by 2
+// roundings of 2^-24 each, the sum and the product by one; the exponent's own roundings make the exponential off by 1.3 |x|
+// more. Where x > 0 that weighs e / (1 + e) < exp(-x), less than half a rounding; where x < 0 it weighs up to 1: within
+// 6 + 1.3 |x| roundings, 2^-19 at x = -20.
 __device__ __forceinline__ float silu16(float x) {
   return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e));
 }
@@ -272,7 +275,9 @@ __global__ __launch_bounds__(64) void causal_conv_kernel(const ActhCausalConvDes
   }
 }
 
-constexpr int CSTEP = 4;                           // 512 sequences x 5120 channels: 1: 24 us, 4: 17, 8: 15
+// sequences a lane, once there are blocks enough: 1, 2, 4, 8 of them in a graph 512 x 5120 16.7, 12.2, 13.0, 14.4 us, 2048 x
+// 5120 54, 36.9, 33.3, 38.0, 300 x 5120 12.2, 9.7, 9.3, 13.6; 128 x 5120 7.3, 6.1, 8.2, 12.7
+constexpr int CSTEP = 4;
 
 // One row a sequence: a lane takes VEC channels of SEQS sequences, whose loads are all under way before the first is
 // used, so that the weights are read once for them. Bound: the kept inputs' bytes; few rows: the launch.
@@ -367,8 +372,9 @@ void launch_conv(const ActhCausalConvDesc& d, hipStream_t stream) {
 // ------------------------------------------------------------------------------------------------ scan
 
 // softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|) in (0, 1]. With w = 1 + e rounded and c = e - (w - 1) what the
-// rounding lost, log1p(e) = log(w) + c / w + ..., and c stands for c / w: they differ by at most 2^-25 e, half a step of
-// the result. So small e keep their digits, which log(1 + e) alone would lose, for 7 operations and two of the slow ones.
+// rounding lost (at most 2^-24), log1p(e) = log(w) + c / w + ..., and c stands for c / w: they differ by at most
+// 2^-24 e / (1 + e), one rounding of the result. So small e keep their digits, which log(1 + e) alone would lose, for 7
+// operations and two of the slow ones.
 __device__ __forceinline__ float softplus16(float x) {
   const float e = __builtin_amdgcn_exp2f(-fabsf(x) * kLog2e);
   const float w = 1.0f + e;
@@ -682,9 +688,10 @@ __global__ __launch_bounds__(64, 3) void ssm_scan_kernel(const ActhSsmScanDesc p
     __syncthreads();
     if (b0 + TT < c1) fetch(b0 + TT);
 
-    // ---- walk its rows (reading the next row's values ahead of their use changed nothing, with many waves or with few)
+    // ---- walk its rows (reading the next row's values ahead of their use changed nothing, with many waves or with few).
+    // Two rows a turn, but where lanes exchange their sums: the compiler leaves that loop whole.
     const int rows = b1 - b0;
-#pragma unroll 2
+#pragma unroll LOCAL || LPC == 1 ? 2 : 1
     for (int r = 0; r < rows; ++r) {
       float B[SPL], y[CPT];
 #pragma unroll
@@ -959,8 +966,8 @@ void launch_step(const ActhSsmScanDesc& d, bool vbc, hipStream_t stream) {
   }
 }
 
-// Few rows and channels: two lanes a channel. 300 x 640: 51 against 45 us, 2000 x 1280: 74 against 70, 16384 x 640: 133
-// against 148.
+// Few rows and channels: two lanes a channel. One against two: 300 x 640 25.1 and 23.3 us, 2000 x 1280 65 and 52, 8192 x 640
+// 91 and 82; 4096 x 2048 96 and 99, 16384 x 640 127 and 130, 8192 x 2560 175 and 208.
 bool scan_small(int N, int T, int D) { return N > 8 && N <= 16 && (long long)T / 64 * ((D + 63) / 64) < 2048; }
 
 // channels a wave takes
@@ -969,7 +976,7 @@ int scan_cb(int N, int T, int D) { return N <= 16 ? (scan_small(N, T, D) ? 32 : 
 // Chunks that give one round of the three waves that fit each of the 1024 SIMDs. Ragged ones, which differ in length, are
 // made half as long (16384 x 5120 in 19 sequences: 775 -> 675 us), but not under 112 rows, where pass 1 leaves out too
 // little (8192 x 2560 in 8: 173 us, of 64 rows 194). Few rows: chunks of 16, each wave being mostly latency (300 x 640 of
-// 64, 32, 16 rows: 45, 31, 25 us).
+// 64, 32, 16 rows: 49, 31, 23 us).
 constexpr int MINLEN = 16;
 Chunks plan(int T, int D, int N, int G, int nseq, int ragged) {
   Chunks c{};
