@@ -113,12 +113,14 @@ __device__ __forceinline__ int4 load16_any(const uint8_t* row, int k, int K) {
 // LDS-DMA. 16-byte chunk c of row r lies at chunk c ^ (r % 8) of its 128-byte LDS row, so the 8 lanes of a ds_read_b128
 // group, which read one chunk of 8 rows, meet 8 different bank slots; the DMA, whose LDS side is linear, applies the
 // same exchange to its global side.
-// Bound: 8192^3 takes 531 us (2070 TFLOP/s; the card's library reaches 2690 with one scale for a whole operand, 1260 in 16
-// bits). The matrix unit is busy 47 % of the time and the vector unit, with the scales' multiply-adds, 38 %, at the
-// 1.9 GHz that the card holds under this load; 17 % of the time goes to the LDS-DMA beside the products and 5 % to the
-// multiply-adds (both timed by leaving them out of a copy). Then rounds of 256 tiles: 16384 x 2560 is 2.5 of them, the last
-// taken as a round of half tiles, at 0.65 of a round's time (238 us, 1800 TFLOP/s at K = 5120; whole tiles 251; a ring of
-// three 256 x 128 stages, five full rounds there, moves twice the bytes a product through L2 and took 275).
+// Bound: 8192^3 takes 531 us (2070 TFLOP/s; the card's library reaches 2690 to 3230, by data and card, with one scale for a
+// whole operand, 1250 to 1590 in 16 bits). Counters at 16384 x 2560 x 5120: the matrix unit is busy 40 % of the time, the vector
+// unit, with the scales' multiply-adds, 36 %, the LDS reads 19 % without a conflict; the waves stand at the end of a block 41 %
+// of their time and wait for an issue slot 29 %. So it is the one barrier a block, behind the LDS-DMA, that two waves a SIMD
+// cannot cover (17 % of the time goes to the DMA beside the products and 5 % to the multiply-adds, both timed by leaving them out
+// of a copy). Then rounds of 256 tiles: 16384 x 2560 is 2.5 of them, the last taken as a round of half tiles, at 0.65 of a
+// round's time (215 - 240 us, 1790 - 2000 TFLOP/s at K = 5120; a ring of three 256 x 128 stages, five full rounds there, moves
+// twice the bytes a product through L2 and took 275).
 template <int BM, int BN>
 struct Tile {
   static constexpr int WC = BN / 64, WR = 8 / WC;              // waves along n and m

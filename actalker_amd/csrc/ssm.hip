@@ -143,16 +143,18 @@ struct ConvLane {
       for (int j = 0; j < W; ++j) w[j][v] = p.w[(long long)(d + v) * W + j];
     }
   }
-  // win: the W - 1 inputs before x, oldest first. EXACT: products and sums rounded one by one in the order of the taps, the
-  // accurate exponential and quotient. A value that lies next to a rounding to 16 bits then falls where the formula's
-  // plain evaluation puts it; a step takes this form, whose result a state of 32 bits keeps (19 against 17.5 us at 512 x
-  // 5120). A prompt's 16-bit outputs are within the same half step by fused sums and the quick quotient, a fused sum being
-  // off by less than the rounded ones (32768 x 5120: 154 against 212 us).
-  template <bool EXACT>
+  // win: the W - 1 inputs before x, oldest first. Two evaluations, both within the fp32 error of the formula, so that their
+  // 16-bit results differ only where the value lies that near a tie. Against 64 bits the fused one (sums by multiply-adds, quick
+  // quotient) falls on the other side of a tie for 2.8e-5 of bf16 values and 1.8e-4 of fp16 ones, the stepwise one (each
+  // product and sum rounded, accurate exponential and quotient) for 4.0e-5 and 2.4e-4. Prompts take the fused one (32768 x 5120:
+  // 154 against 212 us). Steps take the stepwise one, although it costs 1.7 us at 512 x 5120: it is what the formula gives in
+  // fp32 operation by operation, as a program outside these kernels evaluates it, and a state of 32 bits keeps for good what one
+  // 16-bit rounding of its input does (7e-4 of its size at worst in 40 million states; 5e-7 this way).
+  template <bool STEPWISE>
   __device__ __forceinline__ void out(const float (*win)[VEC], const float* x, float* y) const {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-      if constexpr (EXACT) {
+      if constexpr (STEPWISE) {
 #pragma clang fp contract(off)
         float a = w[0][v] * win[0][v];
 #pragma unroll

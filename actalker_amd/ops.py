@@ -1185,7 +1185,8 @@ def causal_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] =
 def causal_conv_step(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, state: torch.Tensor,
                      slots: Optional[torch.Tensor] = None, fresh: Optional[torch.Tensor] = None, silu: bool = True,
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """:func:`causal_conv` of one new token of each sequence: x (n, D), row i belongs to sequence i."""
+    """:func:`causal_conv` of one new token of each sequence: x (n, D), row i belongs to sequence i. A step rounds its sum
+    tap by tap, a prompt fuses it: for the same inputs the two may differ by one rounding to 16 bits."""
     return causal_conv(x, w, bias, nb=x.shape[0], state=state, slots=slots, fresh=fresh, silu=silu, out=out)
 
 
